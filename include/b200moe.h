@@ -274,6 +274,107 @@ int b200moe_pack_int4(const void* w, int out_features, int in_features, int dtyp
 int b200moe_unpack_int4(const void* q, const void* scales, int out_features, int in_features, int dtype,
                         void* q_out, void* w_out, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The attention side of a decoding step and the end of a speculative one.  These entry points need no
+ * context: they run on the current device, allocate nothing, and may run side by side on several streams
+ * as long as outputs and workspaces differ.  `status` (device int32, may be NULL; the caller zeroes it)
+ * collects B200MOE_DEV_* bits of problems that only the device can see.
+ *
+ * Paged cache: k_cache and v_cache [num_blocks, block_size, num_kv_heads, head_dim] with equal strides (the
+ * layout of the reference's PagedKVCache, demo/src/memory/paged_kv_cache.py:228; any page size).  Slot s is
+ * row s % block_size of block s / block_size.  head_dim is 32, 64, 128 or 256 and contiguous; the other
+ * strides, in elements, and all data pointers are multiples of 16 bytes.  f32, f16 or bf16 throughout. */
+
+/* Stores new keys and values into the cache: store_kvcache (demo/src/layers/attention.py:32-79), optionally
+ * with what stands before it in the reference's attention layer, the per-head RMS norms and the rotary
+ * embedding of queries and keys (demo/src/layers/rotary_embedding.py), in the same launch:
+ *   y = x * rsqrt(mean(x^2) + eps) * w      (x where the weight is NULL)
+ *   z = (y1*cos - y2*sin, y2*cos + y1*sin)  (y1, y2: the halves of the head; y where cos_sin is NULL)
+ *   query_out[t] = z(query[t]);  k_cache[slots[t]] = z(key[t]);  v_cache[slots[t]] = value[t]
+ * evaluated in fp32 and rounded once.  query may be NULL (keys and values only); query_out may be query itself.
+ * cos_sin: fp32 [max_position, head_dim], the cosines of a position's head_dim/2 angles, then the sines.
+ * A token with slot -1 stores nothing.  A slot outside the cache (B200MOE_DEV_BAD_SLOT) stores nothing either; a
+ * position outside the table (B200MOE_DEV_BAD_POSITION) stores nothing and gives a query of zeros.  The slots of
+ * one call are distinct: of two tokens with one slot, either may end up there, in whole or in part. */
+typedef struct b200moe_store_kv_args {
+  const void *query, *key, *value;      /* [T, num_heads | num_kv_heads, head_dim], views of a fused projection allowed */
+  void* query_out;
+  void *k_cache, *v_cache;
+  const void *positions, *slots;        /* [T], int64 or int32 as flagged below                     */
+  const float* cos_sin;
+  const void *q_norm_weight, *k_norm_weight; /* [head_dim] in dtype, or NULL                        */
+  int32_t* status;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, o_token_stride, o_head_stride;
+  int64_t cache_block_stride, cache_slot_stride, cache_head_stride;
+  int32_t num_tokens, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_position, dtype;
+  int32_t positions_are_int64, slots_are_int64;
+  float eps;
+  int32_t reserved;
+} b200moe_store_kv_args;
+int b200moe_store_kv(const b200moe_store_kv_args* args, void* stream);
+
+/* Attention of new tokens over the paged cache, which already holds their keys and values: what the reference calls
+ * flash_attn_with_kvcache for, and its per-sequence loop over the spans of a verify batch
+ * (demo/src/layers/attention.py:262-349).  Sequence b owns the query rows query_start[b] .. query_start[b+1]-1 (one
+ * row per sequence where query_start is NULL, then num_tokens == num_seqs); its i-th of n rows sees the first
+ * context_lens[b] - n + i + 1 keys.
+ *   out[t,h] = sum_j softmax_j(scale * q[t,h] . k[j]) v[j];  lse_out[t,h] = log sum_j exp(scale * q . k[j])
+ * A row that sees no key gives zeros and -inf.  Keys that a row does not see do not reach it whatever they hold.
+ * Rows behind query_start[num_seqs] are left as they were.  Page indices outside [0, num_blocks) are not followed
+ * (B200MOE_DEV_BAD_PAGE; that sequence's output is not to be used); lengths that do not fit the tensors are cut, and
+ * spans that do not are skipped (B200MOE_DEV_BAD_LENGTH).
+ * max_query_len: the longest span; longer ones are computed correctly, but read the cache more often.
+ * workspace: as many bytes as b200moe_paged_attention_workspace gives for the same dtype, heads and max_query_len
+ * and for max_context = max_blocks_per_seq * block_size on this device; it need not be cleared and must not be
+ * shared by calls that may overlap.  NULL: sequences are not cut along the cache (slower for long ones). */
+typedef struct b200moe_paged_attention_args {
+  const void* query;                    /* [num_tokens, num_heads, head_dim]                        */
+  const void *k_cache, *v_cache;
+  const int32_t* block_tables;          /* [num_seqs, max_blocks_per_seq], rows block_table_stride apart */
+  const int32_t* context_lens;          /* [num_seqs], the new tokens included                       */
+  const int32_t* query_start;           /* [num_seqs + 1] or NULL                                    */
+  void* out;                            /* [num_tokens, num_heads, head_dim]                         */
+  float* lse_out;                       /* [num_tokens, num_heads] or NULL                           */
+  void* workspace;
+  int32_t* status;
+  int64_t workspace_bytes;
+  int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+  int64_t cache_block_stride, cache_slot_stride, cache_head_stride, block_table_stride;
+  int32_t num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks_per_seq, max_query_len, dtype;
+  float scale;
+  int32_t reserved;
+} b200moe_paged_attention_args;
+int b200moe_paged_attention(const b200moe_paged_attention_args* args, void* stream);
+int b200moe_paged_attention_workspace(int dtype, int num_heads, int num_kv_heads, int head_dim, int max_query_len, int64_t max_context,
+                                      int64_t* bytes_out);
+
+/* Verifies drafted tokens against the target's probabilities by rejection sampling with given random numbers, for all
+ * sequences at once (the engine's _execute_accept is a host loop with a threshold rule,
+ * demo/src/execution/cb_executor.py:261-300).  Sequence b drafted n = draft_start[b+1] - draft_start[b] tokens,
+ * draft_tokens[draft_start[b] ...]; its n + 1 target rows begin at row draft_start[b] + b.
+ *   draft x of position j is accepted while p_j(x) > accept_uniform[j] * q_j(x)   (q = 1 where draft_probs is NULL)
+ *   at the first refusal a token is drawn from max(p_j - q_j, 0) (draft_probs NULL: p_j without x; p_j if nothing is
+ *   left), after n accepted tokens from p_n: the first i with r_0 + ... + r_i > sample_uniform[b] * (r_0 + ... + r_V-1),
+ *   the last i with r_i > 0 if there is none.
+ * Comparisons, differences and sums are in 64 bits; rows need not be normalised; negative values and NaN count as 0.
+ *   tokens_out int64 [num_seqs, max_draft_len + 1]: the accepted tokens, the drawn one, then -1;  accepted_out [num_seqs].
+ * A token outside the vocabulary is refused (B200MOE_DEV_BAD_TOKEN).  Where a row holds nothing to draw from, the drawn
+ * token is -1 (B200MOE_DEV_BAD_PROBS).  A sequence whose numbers do not fit the tensors gets a row of -1 and 0
+ * accepted (B200MOE_DEV_BAD_LENGTH). */
+typedef struct b200moe_verify_draft_args {
+  const int64_t* draft_tokens;          /* [num_draft_tokens]                                        */
+  const void* target_probs;             /* [num_target_rows, vocab_size], rows target_stride apart   */
+  const void* draft_probs;              /* [num_draft_tokens, vocab_size], rows draft_stride apart, or NULL */
+  const float *accept_uniform, *sample_uniform; /* [num_draft_tokens], [num_seqs], in [0,1)         */
+  const int32_t* draft_start;           /* [num_seqs + 1]                                            */
+  int64_t* tokens_out;
+  int32_t* accepted_out;
+  int32_t* status;
+  int64_t target_stride, draft_stride;
+  int32_t num_seqs, vocab_size, max_draft_len, num_draft_tokens, num_target_rows, dtype;
+} b200moe_verify_draft_args;
+int b200moe_verify_draft(const b200moe_verify_draft_args* args, void* stream);
+
 /* Batches of one or two tokens of b200moe_forward_fused / _fused_norm on a dense 16-bit model with ffn_kind AUTO run as ONE
  * cooperative launch that covers router, experts and combine (same results contract as the kernel chain; the
  * expert sums are taken in a different order, so outputs agree to rounding, routing bit for bit).  enable = 0
@@ -288,6 +389,12 @@ int b200moe_status(b200moe_ctx* ctx, int* device_status_out, void* stream);
 #define B200MOE_DEV_BAD_EXPERT_ID 1   /* an id outside [0,E) was supplied; the pair was skipped */
 #define B200MOE_DEV_BAD_OFFSETS 2     /* permute produced inconsistent offsets                   */
 #define B200MOE_DEV_WAIT_EXPIRED 4    /* a bounded on-chip wait gave up                          */
+#define B200MOE_DEV_BAD_SLOT 8        /* a cache slot outside the cache; nothing was stored      */
+#define B200MOE_DEV_BAD_POSITION 16   /* a position outside the angle table                      */
+#define B200MOE_DEV_BAD_PAGE 32       /* a page index outside the cache; it was not followed     */
+#define B200MOE_DEV_BAD_LENGTH 64     /* lengths or offsets that do not fit the tensors          */
+#define B200MOE_DEV_BAD_TOKEN 128     /* a drafted token outside the vocabulary; it was refused  */
+#define B200MOE_DEV_BAD_PROBS 256     /* a row of probabilities with nothing to draw from        */
 
 /* Per-kernel timing for benchmarks.  While enabled, every kernel launch of this context is
  * bracketed by a pair of CUDA events on the launching stream.  b200moe_profile_read waits for

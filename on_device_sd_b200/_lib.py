@@ -22,6 +22,8 @@ EP_HANDLE_BYTES = 64
 KERNEL_CLASSES = 8
 KERNEL_NAMES = ("router", "permute", "ffn_gate_up", "ffn_down", "combine", "ep_dispatch", "ep_return", "token_block")
 ABI_VERSION = 2
+DEV_BAD_EXPERT_ID, DEV_BAD_OFFSETS, DEV_WAIT_EXPIRED = 1, 2, 4
+DEV_BAD_SLOT, DEV_BAD_POSITION, DEV_BAD_PAGE, DEV_BAD_LENGTH, DEV_BAD_TOKEN, DEV_BAD_PROBS = 8, 16, 32, 64, 128, 256
 
 
 class Config(Structure):
@@ -30,6 +32,33 @@ class Config(Structure):
         ("act_dtype", c_int32), ("weight_mode", c_int32), ("num_layers", c_int32), ("max_tokens", c_int32),
         ("device", c_int32), ("reserved", c_int32),
     ]
+
+
+class StoreKvArgs(Structure):
+    _fields_ = ([(n, c_void_p) for n in ("query", "key", "value", "query_out", "k_cache", "v_cache", "positions", "slots", "cos_sin",
+                                         "q_norm_weight", "k_norm_weight", "status")]
+                + [(n, c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride",
+                                          "o_token_stride", "o_head_stride", "cache_block_stride", "cache_slot_stride", "cache_head_stride")]
+                + [(n, c_int32) for n in ("num_tokens", "num_heads", "num_kv_heads", "head_dim", "num_blocks", "block_size", "max_position", "dtype",
+                                          "positions_are_int64", "slots_are_int64")]
+                + [("eps", c_float), ("reserved", c_int32)])
+
+
+class PagedAttentionArgs(Structure):
+    _fields_ = ([(n, c_void_p) for n in ("query", "k_cache", "v_cache", "block_tables", "context_lens", "query_start", "out", "lse_out", "workspace",
+                                         "status")]
+                + [(n, c_int64) for n in ("workspace_bytes", "q_token_stride", "q_head_stride", "o_token_stride", "o_head_stride",
+                                          "cache_block_stride", "cache_slot_stride", "cache_head_stride", "block_table_stride")]
+                + [(n, c_int32) for n in ("num_tokens", "num_seqs", "num_heads", "num_kv_heads", "head_dim", "num_blocks", "block_size",
+                                          "max_blocks_per_seq", "max_query_len", "dtype")]
+                + [("scale", c_float), ("reserved", c_int32)])
+
+
+class VerifyDraftArgs(Structure):
+    _fields_ = ([(n, c_void_p) for n in ("draft_tokens", "target_probs", "draft_probs", "accept_uniform", "sample_uniform", "draft_start", "tokens_out",
+                                         "accepted_out", "status")]
+                + [(n, c_int64) for n in ("target_stride", "draft_stride")]
+                + [(n, c_int32) for n in ("num_seqs", "vocab_size", "max_draft_len", "num_draft_tokens", "num_target_rows", "dtype")])
 
 
 # name -> (restype, argtypes); every symbol include/b200moe.h declares
@@ -67,6 +96,10 @@ PROTOTYPES = {
     "b200moe_group_pairs": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "b200moe_pack_int4": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "b200moe_unpack_int4": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "b200moe_store_kv": (c_int, [POINTER(StoreKvArgs), c_void_p]),
+    "b200moe_paged_attention": (c_int, [POINTER(PagedAttentionArgs), c_void_p]),
+    "b200moe_paged_attention_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int64, POINTER(c_int64)]),
+    "b200moe_verify_draft": (c_int, [POINTER(VerifyDraftArgs), c_void_p]),
     "b200moe_profile": (c_int, [c_void_p, c_int]),
     "b200moe_profile_read": (c_int, [c_void_p, c_void_p, c_void_p]),
     "b200moe_set_token_kernel": (c_int, [c_void_p, c_int]),

@@ -1,0 +1,279 @@
+// C entry points of the attention side of a decoding step: b200moe_store_kv, b200moe_paged_attention.
+#include "../../include/b200moe.h"
+
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+#include "common.cuh"
+#include "internal.h"
+#include "kv_store.cuh"
+#include "paged_attention.cuh"
+
+using namespace b200moe;
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+bool unaligned(const void* p) { return ((uintptr_t)p & 15u) != 0; }
+size_t elem_bytes(int dtype) { return dtype == B200MOE_F32 ? 4 : 2; }
+bool odd_stride(int64_t s, int dtype) { return ((size_t)s * elem_bytes(dtype)) % 16 != 0; }
+bool known_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
+
+int current_device(const char* who, int* dev) {
+  cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return b200moe_fail_global(B200MOE_E_CUDA, "%s: no CUDA device: %s (there is no CPU path)", who, cudaGetErrorString(e));
+  if (*dev < 0 || *dev >= kMaxDevices) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: device ordinal %d not supported", who, *dev);
+  return B200MOE_OK;
+}
+
+// Every kernel here waits for its predecessor itself (pdl_wait), so it may be launched while that one drains.
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// ---------------------------------------------------------------------------------------------
+// b200moe_store_kv
+// ---------------------------------------------------------------------------------------------
+template <typename T, int D> cudaError_t launch_store(const StoreKvParams& p, cudaStream_t s) {
+  constexpr int L = D / 16;
+  const int heads = p.Hq + 2 * p.Hkv;
+  // One head per lane group until that fills the GPU about twice (148 SMs x 2048 threads), four from there on.
+  const bool wide = (long long)p.T * heads * L >= 2ll * 148 * 2048;
+  const long long groups = (long long)p.T * (wide ? (heads + 3) / 4 : heads);
+  const unsigned grid = (unsigned)((groups * L + kStoreThreads - 1) / kStoreThreads);
+  return wide ? launch(store_kv_kernel<T, D, 4>, grid, kStoreThreads, 0, s, p) : launch(store_kv_kernel<T, D, 1>, grid, kStoreThreads, 0, s, p);
+}
+template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, cudaStream_t s) {
+  switch (D) {
+    case 32: return launch_store<T, 32>(p, s);
+    case 64: return launch_store<T, 64>(p, s);
+    case 128: return launch_store<T, 128>(p, s);
+    default: return launch_store<T, 256>(p, s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// b200moe_paged_attention
+// ---------------------------------------------------------------------------------------------
+// Up to this many cache slots per sequence (pages x page size) a unit is not cut: joining its parts would cost a second
+// launch, about as long as one CTA needs for them.
+constexpr long long kNoSplitSlots = 256;
+
+struct AttnPlan {
+  int grid = 0, R = 0;
+  int64_t ws_bytes = 0;
+};
+
+template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB> struct AttnVariant {
+  using S = AttnShape<T, D, MT, RG, KG, STAGES>;
+  // CTAs that fill the device, kept per device; 0 = not asked yet.  Two threads that ask at once store the same number.
+  static int fill(int dev, cudaError_t* err) {
+    static std::atomic<int> known[kMaxDevices];
+    int n = known[dev].load(std::memory_order_acquire);
+    if (n) return n;
+    auto k = attn_kernel<T, D, MT, RG, KG, STAGES, MINB>;
+    int per_sm = 0, sms = 0;
+    *err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (*err == cudaSuccess) *err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, S::THREADS, S::SMEM);
+    if (*err == cudaSuccess) *err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (*err != cudaSuccess) return 0;
+    n = per_sm * sms;
+    if (n <= 0) { *err = cudaErrorLaunchOutOfResources; return 0; }
+    known[dev].store(n, std::memory_order_release);
+    return n;
+  }
+  static cudaError_t run(AttnParams* p, int dev, AttnPlan* plan, cudaStream_t s, bool plan_only) {
+    cudaError_t e = cudaSuccess;
+    plan->grid = fill(dev, &e);
+    if (e != cudaSuccess) return e;
+    plan->R = S::R;
+    plan->ws_bytes = 2ll * plan->grid * S::R * (D + 2) * 4;
+    if (plan_only) return cudaSuccess;
+    p->grid = plan->grid;
+    p->tile = S::TILE;
+    e = launch(attn_kernel<T, D, MT, RG, KG, STAGES, MINB>, (unsigned)plan->grid, S::THREADS, S::SMEM, s, *p);
+    if (e != cudaSuccess || !p->split) return e;
+    const long long rows = (long long)p->T * p->Hq;
+    // Few rows are cut into many parts each: eight warps per row.  Many rows: one warp, or the launch grows.
+    if (rows <= 148 * 8) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R);
+    return launch(attn_join_kernel<T, D, 1>, (unsigned)((rows + 7) / 8), 256, 0, s, *p, S::R);
+  }
+};
+
+// Rows that share a kv head's keys: tokens of the span x query heads of the group.  The smallest tile that holds them,
+// at most 64 (32 for heads of 256): more rows than that read the cache once per tile.
+template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int rows, int dev, AttnPlan* plan, cudaStream_t s, bool po) {
+  if constexpr (sizeof(T) == 4) {
+    switch (D) {
+      case 32: return AttnVariant<T, 32, 1, 1, 4, 4, 2>::run(p, dev, plan, s, po);
+      case 64: return AttnVariant<T, 64, 1, 1, 4, 3, 2>::run(p, dev, plan, s, po);
+      case 128: return AttnVariant<T, 128, 1, 1, 4, 3, 1>::run(p, dev, plan, s, po);
+      default: return AttnVariant<T, 256, 1, 1, 2, 3, 1>::run(p, dev, plan, s, po);
+    }
+  } else {
+    switch (D) {
+      case 32:
+        if (rows <= 16) return AttnVariant<T, 32, 1, 1, 4, 6, 4>::run(p, dev, plan, s, po);
+        if (rows <= 32) return AttnVariant<T, 32, 2, 1, 4, 6, 3>::run(p, dev, plan, s, po);
+        return AttnVariant<T, 32, 2, 2, 4, 6, 2>::run(p, dev, plan, s, po);
+      case 64:
+        if (rows <= 16) return AttnVariant<T, 64, 1, 1, 4, 4, 3>::run(p, dev, plan, s, po);
+        if (rows <= 32) return AttnVariant<T, 64, 2, 1, 4, 4, 3>::run(p, dev, plan, s, po);
+        return AttnVariant<T, 64, 2, 2, 4, 5, 2>::run(p, dev, plan, s, po);
+      case 128:
+        if (rows <= 16) return AttnVariant<T, 128, 1, 1, 4, 3, 2>::run(p, dev, plan, s, po);
+        if (rows <= 32) return AttnVariant<T, 128, 2, 1, 4, 3, 2>::run(p, dev, plan, s, po);
+        return AttnVariant<T, 128, 2, 2, 4, 6, 1>::run(p, dev, plan, s, po);
+      default:
+        if (rows <= 16) return AttnVariant<T, 256, 1, 1, 4, 3, 1>::run(p, dev, plan, s, po);
+        return AttnVariant<T, 256, 1, 2, 4, 3, 1>::run(p, dev, plan, s, po);
+    }
+  }
+}
+
+int run_attn(AttnParams* p, int dtype, int D, int rows, int dev, AttnPlan* plan, cudaStream_t s, bool plan_only, const char* who) {
+  cudaError_t e;
+  switch (dtype) {
+    case B200MOE_F32: e = dispatch_attn<float>(p, D, rows, dev, plan, s, plan_only); break;
+    case B200MOE_F16: e = dispatch_attn<__half>(p, D, rows, dev, plan, s, plan_only); break;
+    default: e = dispatch_attn<__nv_bfloat16>(p, D, rows, dev, plan, s, plan_only); break;
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return b200moe_fail_global(B200MOE_E_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+  }
+  return B200MOE_OK;
+}
+
+int check_heads(const char* who, int dtype, int Hq, int Hkv, int D) {
+  if (dtype < B200MOE_F32 || dtype > B200MOE_BF16) return b200moe_fail_global(B200MOE_E_ARG, "%s: unknown dtype %d", who, dtype);
+  if (!known_head_dim(D)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: head_dim %d (32, 64, 128 or 256)", who, D);
+  if (Hq <= 0 || Hkv <= 0 || Hq > 65536 || Hkv > 65536) return b200moe_fail_global(B200MOE_E_ARG, "%s: head counts must be in 1..65536", who);
+  if (Hq % Hkv) return b200moe_fail_global(B200MOE_E_ARG, "%s: %d query heads are not a multiple of %d key-value heads", who, Hq, Hkv);
+  return B200MOE_OK;
+}
+
+}  // namespace
+
+extern "C" int b200moe_store_kv(const b200moe_store_kv_args* a, void* stream) {
+  const char* who = "b200moe_store_kv";
+  if (!a) return b200moe_fail_global(B200MOE_E_ARG, "%s: null arguments", who);
+  const bool has_q = a->query != nullptr;
+  const int dt = a->dtype;
+  if (int rc = check_heads(who, dt, has_q ? a->num_heads : a->num_kv_heads, a->num_kv_heads, a->head_dim)) return rc;
+  if (a->num_tokens < 0 || a->num_blocks < 0 || a->block_size <= 0) return b200moe_fail_global(B200MOE_E_ARG, "%s: negative size", who);
+  if (a->num_tokens == 0) return B200MOE_OK;
+  if (!a->key || !a->value || !a->k_cache || !a->v_cache || !a->slots) return b200moe_fail_global(B200MOE_E_ARG, "%s: null pointer", who);
+  if (has_q && !a->query_out) return b200moe_fail_global(B200MOE_E_ARG, "%s: query given without query_out", who);
+  if (a->cos_sin && (!a->positions || a->max_position <= 0)) return b200moe_fail_global(B200MOE_E_ARG, "%s: an angle table needs positions and its length", who);
+  const void* ptrs[] = {a->query, a->key, a->value, a->query_out, a->k_cache, a->v_cache, a->cos_sin, a->q_norm_weight, a->k_norm_weight};
+  for (const void* p : ptrs)
+    if (unaligned(p)) return b200moe_fail_global(B200MOE_E_ARG, "%s: data pointers must be 16-byte aligned", who);
+  const int64_t strides[] = {a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride,
+                             a->o_token_stride, a->o_head_stride, a->cache_block_stride, a->cache_slot_stride, a->cache_head_stride};
+  for (int64_t s : strides)
+    if (odd_stride(s, dt)) return b200moe_fail_global(B200MOE_E_ARG, "%s: strides must be multiples of 16 bytes", who);
+  if ((int64_t)a->num_tokens * (a->num_heads + 2ll * a->num_kv_heads) > (1ll << 36)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: too many heads x tokens", who);
+  int dev;
+  if (int rc = current_device(who, &dev)) return rc;
+  StoreKvParams p = {};
+  p.q = a->query; p.k = a->key; p.v = a->value; p.q_out = a->query_out; p.k_cache = a->k_cache; p.v_cache = a->v_cache;
+  p.positions = a->positions; p.slots = a->slots; p.cos_sin = a->cos_sin; p.q_weight = has_q ? a->q_norm_weight : nullptr; p.k_weight = a->k_norm_weight;
+  p.status = a->status;
+  p.q_tok = a->q_token_stride; p.q_head = a->q_head_stride; p.k_tok = a->k_token_stride; p.k_head = a->k_head_stride;
+  p.v_tok = a->v_token_stride; p.v_head = a->v_head_stride; p.o_tok = a->o_token_stride; p.o_head = a->o_head_stride;
+  p.c_block = a->cache_block_stride; p.c_slot = a->cache_slot_stride; p.c_head = a->cache_head_stride;
+  p.num_slots = (long long)a->num_blocks * a->block_size;
+  p.T = a->num_tokens; p.Hq = has_q ? a->num_heads : 0; p.Hkv = a->num_kv_heads; p.block_size = a->block_size; p.max_position = a->max_position;
+  p.positions64 = a->positions_are_int64; p.slots64 = a->slots_are_int64; p.eps = a->eps;
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e;
+  switch (dt) {
+    case B200MOE_F32: e = dispatch_store<float>(p, a->head_dim, s); break;
+    case B200MOE_F16: e = dispatch_store<__half>(p, a->head_dim, s); break;
+    default: e = dispatch_store<__nv_bfloat16>(p, a->head_dim, s); break;
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return b200moe_fail_global(B200MOE_E_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+  }
+  return B200MOE_OK;
+}
+
+extern "C" int b200moe_paged_attention_workspace(int dtype, int num_heads, int num_kv_heads, int head_dim, int max_query_len, int64_t max_context,
+                                                 int64_t* bytes_out) {
+  const char* who = "b200moe_paged_attention_workspace";
+  if (!bytes_out) return b200moe_fail_global(B200MOE_E_ARG, "%s: null pointer", who);
+  if (int rc = check_heads(who, dtype, num_heads, num_kv_heads, head_dim)) return rc;
+  if (max_query_len < 0 || max_context < 0) return b200moe_fail_global(B200MOE_E_ARG, "%s: negative size", who);
+  *bytes_out = 0;
+  if (max_context <= kNoSplitSlots) return B200MOE_OK;
+  int dev;
+  if (int rc = current_device(who, &dev)) return rc;
+  AttnPlan plan;
+  const long long rows = (long long)max_query_len * (num_heads / num_kv_heads);
+  if (int rc = run_attn(nullptr, dtype, head_dim, (int)(rows < 1024 ? rows : 1024), dev, &plan, nullptr, true, who)) return rc;
+  *bytes_out = plan.ws_bytes;
+  return B200MOE_OK;
+}
+
+extern "C" int b200moe_paged_attention(const b200moe_paged_attention_args* a, void* stream) {
+  const char* who = "b200moe_paged_attention";
+  if (!a) return b200moe_fail_global(B200MOE_E_ARG, "%s: null arguments", who);
+  const int dt = a->dtype;
+  if (int rc = check_heads(who, dt, a->num_heads, a->num_kv_heads, a->head_dim)) return rc;
+  if (a->num_tokens < 0 || a->num_seqs < 0 || a->num_blocks < 0 || a->block_size <= 0 || a->max_blocks_per_seq < 0 || a->max_query_len < 0)
+    return b200moe_fail_global(B200MOE_E_ARG, "%s: negative size", who);
+  if (!a->query_start && a->num_tokens != a->num_seqs)
+    return b200moe_fail_global(B200MOE_E_ARG, "%s: without query_start there is one token per sequence (%d tokens, %d sequences)", who, a->num_tokens, a->num_seqs);
+  if (a->num_tokens == 0 || a->num_seqs == 0) return B200MOE_OK;
+  const bool has_cache = a->num_blocks > 0 && a->max_blocks_per_seq > 0;
+  if (!a->query || !a->out || !a->context_lens || (has_cache && (!a->k_cache || !a->v_cache || !a->block_tables)))
+    return b200moe_fail_global(B200MOE_E_ARG, "%s: null pointer", who);
+  if (unaligned(a->query) || unaligned(a->out) || unaligned(a->k_cache) || unaligned(a->v_cache) || unaligned(a->workspace))
+    return b200moe_fail_global(B200MOE_E_ARG, "%s: data pointers must be 16-byte aligned", who);
+  const int64_t strides[] = {a->q_token_stride, a->q_head_stride, a->o_token_stride, a->o_head_stride, a->cache_block_stride, a->cache_slot_stride,
+                             a->cache_head_stride};
+  for (int64_t s : strides)
+    if (odd_stride(s, dt)) return b200moe_fail_global(B200MOE_E_ARG, "%s: strides must be multiples of 16 bytes", who);
+  if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return b200moe_fail_global(B200MOE_E_ARG, "%s: scale must be positive and finite", who);
+  const int64_t max_context = (int64_t)a->max_blocks_per_seq * a->block_size;
+  if (max_context > (1ll << 30)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: block tables span more than 2^30 slots", who);
+  // the join's grid and the row numbers are 32-bit
+  if ((int64_t)a->num_tokens * a->num_heads > (1ll << 30)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: more than 2^30 tokens x heads", who);
+  int dev;
+  if (int rc = current_device(who, &dev)) return rc;
+  AttnParams p = {};
+  p.q = a->query; p.k = a->k_cache; p.v = a->v_cache; p.out = a->out; p.lse = a->lse_out;
+  p.tables = a->block_tables; p.context = a->context_lens; p.qstart = a->query_start; p.status = a->status; p.ws = (float*)a->workspace;
+  p.q_tok = a->q_token_stride; p.q_head = a->q_head_stride; p.o_tok = a->o_token_stride; p.o_head = a->o_head_stride;
+  p.c_block = a->cache_block_stride; p.c_slot = a->cache_slot_stride; p.c_head = a->cache_head_stride; p.table_stride = a->block_table_stride;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.B = a->num_seqs; p.T = a->num_tokens; p.Hq = a->num_heads; p.Hkv = a->num_kv_heads; p.group = a->num_heads / a->num_kv_heads;
+  p.block_size = a->block_size; p.num_blocks = a->num_blocks; p.max_blocks = a->max_blocks_per_seq;
+  const long long span = a->query_start ? a->max_query_len : 1;
+  const long long rows = span * p.group;
+  AttnPlan plan;
+  const int rows_i = (int)(rows < 1024 ? rows : 1024);
+  p.split = max_context > kNoSplitSlots && a->workspace != nullptr;
+  if (p.split) {
+    if (int rc = run_attn(&p, dt, a->head_dim, rows_i, dev, &plan, nullptr, true, who)) return rc;
+    if (a->workspace_bytes < plan.ws_bytes)
+      return b200moe_fail_global(B200MOE_E_ARG, "%s: workspace of %lld bytes, %lld are needed (b200moe_paged_attention_workspace)", who,
+                                 (long long)a->workspace_bytes, (long long)plan.ws_bytes);
+  }
+  return run_attn(&p, dt, a->head_dim, rows_i, dev, &plan, (cudaStream_t)stream, false, who);
+}

@@ -158,5 +158,11 @@ __device__ __forceinline__ bool ep_wait_flag(const unsigned* flag, unsigned epoc
 constexpr int kDevBadExpertId = 1;
 constexpr int kDevBadOffsets = 2;
 constexpr int kDevWaitExpired = 4;
+constexpr int kDevBadSlot = 8;
+constexpr int kDevBadPosition = 16;
+constexpr int kDevBadPage = 32;
+constexpr int kDevBadLength = 64;
+constexpr int kDevBadToken = 128;
+constexpr int kDevBadProbs = 256;
 
 }  // namespace b200moe

@@ -1,0 +1,662 @@
+// Attention of one or a few new tokens per sequence over a paged key-value cache (what the reference calls
+// flash_attn_with_kvcache and its per-sequence fallback for, demo/src/layers/attention.py:262-349):
+//
+//   o[t,h] = sum_j softmax_j(scale * q[t,h] . k[j,g]) v[j,g],   g = h / (Hq/Hkv),   j < limit(t)
+//   limit(t) = context - n + i + 1     for the i-th of a sequence's n new tokens (the cache already holds them)
+//
+// One pass over the cache with the running maximum and sum of a softmax.  What bounds it is HBM: a key and a value are
+// read once for all query heads of their group and all tokens of the span (rows), 2 flops per row and byte.
+//
+// Work split.  A unit is (sequence, tile of R rows, kv head); it is cut along the cache into tiles of 64 keys (32 for
+// the widest fp32 heads), and the
+// tiles of all units, laid end to end, are dealt to the CTAs in equal contiguous ranges computed from the lengths on
+// the device, so ragged batches stay balanced without the host knowing a length.  A CTA that holds a whole unit writes
+// the output; otherwise it leaves (m, l, o) of its part in the workspace and attn_join_kernel joins the parts in
+// index order (results do not depend on timing).
+//
+// Inside a CTA four key groups take 16 of the 64 keys of a tile each, with a ring of shared memory of their own that
+// they fill with cp.async: no barrier of the CTA in the loop (with two row groups, one of 64 threads per stage).
+// 16-bit types multiply on mma.sync m16n8k16: rows (padded to 16) x keys, accumulators and the softmax in registers.
+// At 16..64 rows the tensor pipe is far from full even so (about a fifth busy at 16 rows when HBM is saturated), and
+// the hand-over through tensor memory that tcgen05 needs between the two products would be the longer path.
+// fp32 multiplies on the CUDA cores.
+//
+// Roundings: scores, softmax, sums and accumulators are fp32; p is rounded to the cache's type for the second product
+// (the operand type of the tensor cores; the sum l uses the same unrounded p), outputs are rounded once.
+#pragma once
+#include "common.cuh"
+#include "tma.cuh"
+
+namespace b200moe {
+
+struct AttnParams {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;                      // may be null
+  const int* tables;               // [B, table_stride]
+  const int* context;              // [B]
+  const int* qstart;               // [B+1] or null: one token per sequence
+  int* status;                     // may be null
+  float* ws;                       // parts: [2 * grid][R * D] o, then [2 * grid][R][2] (m, l)
+  long long q_tok, q_head, o_tok, o_head, c_block, c_slot, c_head, table_stride;
+  float scale_log2;                // scale * log2(e)
+  int B, T, Hq, Hkv, group, block_size, num_blocks, max_blocks;
+  int split;                       // 0: units are not cut
+  int tile;                        // keys of a tile
+  int grid;                        // CTAs of the attention kernel
+};
+
+// ---------------------------------------------------------------------------------------------
+// The work list, as every thread can recompute it from the lengths
+// ---------------------------------------------------------------------------------------------
+struct AttnSeq {
+  int first, n, ctx;               // first query row, new tokens, keys
+  int row_tiles, tiles;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b, int R) {
+  AttnSeq s;
+  s.first = b; s.n = 1;
+  s.ctx = p.context[b];
+  if (p.qstart) {
+    s.first = p.qstart[b];
+    s.n = p.qstart[b + 1] - s.first;
+  }
+  // lengths that do not fit the tensors: nothing is read or written out of range (reported by attn_report)
+  if (s.first < 0 || s.n < 0 || s.first > p.T || s.n > p.T - s.first) s.n = 0;
+  const long long cap = (long long)p.max_blocks * p.block_size;
+  if (s.ctx < 0) s.ctx = 0;
+  if (s.ctx > cap) s.ctx = (int)cap;
+  s.row_tiles = (s.n * p.group + R - 1) / R;
+  s.tiles = max((s.ctx + p.tile - 1) / p.tile, 1);   // an empty sequence still has rows to write
+  return s;
+}
+__device__ __forceinline__ void attn_report(const AttnParams& p, int b) {
+  if (!p.status) return;
+  bool bad = p.context[b] < 0 || p.context[b] > (long long)p.max_blocks * p.block_size;
+  if (p.qstart) {
+    const int f = p.qstart[b], e = p.qstart[b + 1];
+    bad = bad || f < 0 || e < f || e > p.T;
+  }
+  if (bad) atomicOr(p.status, kDevBadLength);
+}
+__device__ __forceinline__ long long attn_work(const AttnParams& p, const AttnSeq& s) {
+  return (long long)s.row_tiles * p.Hkv * (p.split ? s.tiles : 1);
+}
+__device__ __forceinline__ long long warp_sum_ll(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Work of the sequences [0, b_end), by a whole warp.
+__device__ __forceinline__ long long attn_work_before(const AttnParams& p, int b_end, int R) {
+  long long w = 0;
+  for (int b = threadIdx.x & 31; b < b_end; b += 32) w += attn_work(p, attn_seq(p, b, R));
+  return warp_sum_ll(w);
+}
+// The sequence that holds work item x, and the work before it; by a whole warp.
+__device__ __forceinline__ int attn_find(const AttnParams& p, long long x, int R, long long* before) {
+  const int lane = threadIdx.x & 31;
+  long long base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    const long long w = b < p.B ? attn_work(p, attn_seq(p, b, R)) : 0;
+    long long inc = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, x < base + inc);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      *before = base + __shfl_sync(0xffffffffu, inc - w, src);
+      return b0 + src;
+    }
+    base += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  *before = base;
+  return p.B;
+}
+// CTA c of g takes the items [attn_lo(c), attn_lo(c+1)); item x belongs to CTA attn_owner(x).  g <= W.
+__device__ __forceinline__ long long attn_lo(long long W, int g, int c) { return W * c / g; }
+__device__ __forceinline__ int attn_owner(long long W, int g, long long x) { return (int)(((x + 1) * g - 1) / W); }
+
+// ---------------------------------------------------------------------------------------------
+// Primitives
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  // a source size of zero fills the 16 bytes with zeros and reads nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T> __device__ __forceinline__ bool any_nonfinite2(uint32_t x) {   // either of two packed 16-bit values
+  const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (x & e) == e || ((x >> 16) & e) == e;
+}
+
+// Rows of ROWB bytes; 16-byte chunks are permuted within a row so that the eight rows that an ldmatrix or a quarter
+// warp reads at one chunk position lie in eight different bank groups.
+template <int ROWB> __device__ __forceinline__ uint32_t row_chunk(int row, int chunk) {
+  if constexpr (ROWB >= 128) return row * ROWB + ((chunk ^ (row & 7)) << 4);
+  else return row * ROWB + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+// MT: 16-row tiles of a warp, RG: row groups (warps that share a ring), KG: key groups.
+template <typename T, int D, int MT, int RG, int KG, int STAGES_> struct AttnShape {
+  static constexpr int R = 16 * MT * RG;
+  static constexpr int STAGES = STAGES_;
+  static constexpr int KEYS = 16;                  // keys of a stage
+  static constexpr int TILE = KEYS * KG;
+  static constexpr int THREADS = 32 * KG * RG;
+  static constexpr int ROWB = D * (int)sizeof(T);
+  static constexpr int CPR = ROWB / 16;
+  static constexpr int HALF_STAGE = KEYS * ROWB;   // K, then V
+  static constexpr int RING = KG * STAGES * 2 * HALF_STAGE;
+  static constexpr int JOIN = KG * R * D * 4;      // the key groups' o, in the ring's place
+  static constexpr int MAIN = RING > JOIN ? RING : JOIN;
+  static constexpr int Q_OFF = MAIN;
+  static constexpr int ML_OFF = Q_OFF + R * ROWB;
+  static constexpr int P_OFF = ML_OFF + KG * R * 8;                        // fp32 only: p [KG][KEYS][16], factors [KG][16]
+  static constexpr int SMEM = P_OFF + (sizeof(T) == 4 ? KG * (KEYS + 1) * 16 * 4 : 0);
+};
+
+template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB>
+__global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnParams p) {
+  using S = AttnShape<T, D, MT, RG, KG, STAGES>;
+  constexpr int R = S::R, ROWB = S::ROWB, CPR = S::CPR, KEYS = S::KEYS, THREADS = S::THREADS;
+  constexpr bool kMma = sizeof(T) == 2;
+  static_assert(kMma ? KEYS == 16 : (MT == 1 && RG == 1 && KEYS <= 32), "shape");
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kg = warp % KG, rg = warp / KG;
+  const uint32_t sbase = smem_addr(smem);
+  const uint32_t ring = sbase + kg * (STAGES * 2 * S::HALF_STAGE);
+  float* s_o = reinterpret_cast<float*>(smem);
+  float2* s_ml = reinterpret_cast<float2*>(smem + S::ML_OFF);
+
+  pdl_trigger();
+  pdl_wait();
+  if (p.status)
+    for (int b = blockIdx.x * THREADS + tid; b < p.B; b += gridDim.x * THREADS) attn_report(p, b);
+  const long long W = attn_work_before(p, p.B, R);
+  const int g = (int)(W < p.grid ? W : p.grid);
+  const int cta = blockIdx.x;
+  if (cta >= g) return;
+  long long lo = attn_lo(W, g, cta);
+  const long long my_lo = lo, hi = attn_lo(W, g, cta + 1);
+  long long seq_base;
+  int b = attn_find(p, lo, R, &seq_base);
+  const T* kc = reinterpret_cast<const T*>(p.k);
+  const T* vc = reinterpret_cast<const T*>(p.v);
+
+  while (lo < hi && b < p.B) {
+    const AttnSeq sq = attn_seq(p, b, R);
+    const long long seq_work = attn_work(p, sq);
+    if (lo >= seq_base + seq_work) { seq_base += seq_work; ++b; continue; }
+    const int weight = p.split ? sq.tiles : 1;
+    const int unit = (int)((lo - seq_base) / weight);
+    const int skip = (int)((lo - seq_base) % weight);                 // tiles of this unit that other CTAs took
+    const long long left = hi - lo;
+    const int tile0 = skip;
+    const int ntile = p.split ? (int)(left < weight - skip ? left : weight - skip) : sq.tiles;
+    const bool whole = !p.split || (skip == 0 && ntile == weight);
+    const int slot = 2 * cta + (lo == my_lo && skip > 0 ? 0 : 1);
+    lo += p.split ? ntile : 1;
+    const int rt = unit / p.Hkv, head = unit % p.Hkv;
+    const int row0 = rt * R, rows = min(R, sq.n * p.group - row0);    // rows of the sequence: token-major, then head of the group
+
+    // --- loads of the cache: the 16 lanes of a row fetch its chunks; lane j < KEYS knows where key j of the stage lies
+    const int* table = p.tables + (long long)b * p.table_stride;
+    const T* kh = kc + head * p.c_head;
+    const T* vh = vc + head * p.c_head;
+    int page_next = 0;
+    auto lookup = [&](int t) {                                        // page of this lane's key of tile t (one stage ahead)
+      const int key = (tile0 + t) * S::TILE + kg * KEYS + (lane % KEYS);
+      page_next = (t < ntile && key < sq.ctx) ? __ldg(table + key / p.block_size) : -1;
+    };
+    auto issue = [&](int t) {
+      if (t < ntile) {
+        const int key = (tile0 + t) * S::TILE + kg * KEYS + (lane % KEYS);
+        const bool in = key < sq.ctx;
+        const bool ok = in && page_next >= 0 && page_next < p.num_blocks;
+        if (in && !ok && p.status) atomicOr(p.status, kDevBadPage);
+        const long long off = ok ? page_next * p.c_block + (long long)(key % p.block_size) * p.c_slot : -1;
+        const uint32_t dst = ring + (t % STAGES) * (2 * S::HALF_STAGE);
+        const int pt = rg * 32 + lane;
+        constexpr int STEP = 32 * RG;
+#pragma unroll
+        for (int i = 0; i < (KEYS * CPR + STEP - 1) / STEP; ++i) {
+          const int idx = pt + i * STEP;
+          const int row = idx / CPR, ch = idx % CPR;
+          const long long o = __shfl_sync(0xffffffffu, off, row % KEYS);
+          if (KEYS * CPR % STEP == 0 || idx < KEYS * CPR) {
+            const long long e = (o < 0 ? 0 : o) + ch * (16 / (int)sizeof(T));
+            const uint32_t d = dst + row_chunk<ROWB>(row, ch);
+            cp_async16(d, kh + e, o >= 0);
+            cp_async16(d + S::HALF_STAGE, vh + e, o >= 0);
+          }
+        }
+        lookup(t + 1);
+      }
+      cp_async_commit();
+    };
+    lookup(0);
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) issue(t);
+
+    // --- queries
+    for (int i = tid; i < R * CPR; i += THREADS) {
+      const int r = i / CPR, ch = i % CPR;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int token = sq.first + (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
+        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + token * p.q_tok + h * p.q_head + ch * (16 / (int)sizeof(T)));
+      }
+      *reinterpret_cast<uint4*>(smem + S::Q_OFF + row_chunk<ROWB>(r, ch)) = x;
+    }
+    __syncthreads();
+
+    const int lim0 = sq.ctx - sq.n + 1 + row0 / p.group;              // keys that the first (and least seeing) row sees
+    auto limit = [&](int r) { return sq.ctx - sq.n + 1 + (row0 + min(r, rows - 1)) / p.group; };
+
+    if constexpr (kMma) {
+      // rows lane/4 and lane/4 + 8 of each 16-row tile, columns 2*(lane%4), +1 of each 8-column tile
+      float o[MT][D / 8][4];
+      float m[MT][2], l[MT][2];
+      int lim[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.0f;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          m[mt][hh] = -INFINITY; l[mt][hh] = 0.0f;
+          lim[mt][hh] = limit(rg * 16 * MT + mt * 16 + hh * 8 + (lane >> 2));
+        }
+      }
+      const uint32_t qbase = sbase + S::Q_OFF;
+      const int qrow = rg * 16 * MT + (lane & 7) + ((lane >> 3) & 1) * 8, qch = lane >> 4;
+      const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
+      const int vrow = (lane & 7) + ((lane >> 3) & 1) * 8, vch = lane >> 4;
+      constexpr bool kQRegs = MT == 1 && D <= 128;                    // else the registers are needed for o
+      uint32_t qf[kQRegs ? D / 16 : 1][4];
+      if constexpr (kQRegs) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) ldsm4(qf[ks], qbase + row_chunk<ROWB>(qrow, 2 * ks + qch));
+      }
+
+      for (int t = 0; t < ntile; ++t) {
+        cp_async_wait<STAGES - 2>();
+        if constexpr (RG > 1) bar_sync(1 + kg, 32 * RG); else __syncwarp();
+        issue(t + STAGES - 1);
+        const uint32_t ks_base = ring + (t % STAGES) * (2 * S::HALF_STAGE), vs_base = ks_base + S::HALF_STAGE;
+        const int key0 = (tile0 + t) * S::TILE + kg * KEYS;
+        if (key0 >= sq.ctx) continue;                                 // nothing of the last tile in this group
+
+        float s[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t kf[4];
+          ldsm4(kf, ks_base + row_chunk<ROWB>(krow, 2 * ks + kch));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            if constexpr (kQRegs) {
+              mma16816<T>(s[mt][0], qf[ks], kf[0], kf[1]);
+              mma16816<T>(s[mt][1], qf[ks], kf[2], kf[3]);
+            } else {
+              uint32_t a[4];
+              ldsm4(a, qbase + row_chunk<ROWB>(qrow + mt * 16, 2 * ks + qch));
+              mma16816<T>(s[mt][0], a, kf[0], kf[1]);
+              mma16816<T>(s[mt][1], a, kf[2], kf[3]);
+            }
+          }
+        }
+
+        const bool masked = key0 + KEYS > lim0;
+        uint32_t pf[MT][4];
+        bool grew = false;
+        float fac[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + (i >> 1) * 8 + 2 * (lane & 3) + (i & 1);
+              x[i] = s[mt][i >> 1][2 * hh + (i & 1)] * p.scale_log2;
+              if (masked && key >= lim[mt][hh]) x[i] = -INFINITY;
+            }
+            float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float mn = fmaxf(m[mt][hh], top);
+            const float ref = mn == -INFINITY ? 0.0f : mn;            // a row that has seen nothing yet
+            fac[mt][hh] = exp2f(m[mt][hh] - ref);
+            grew = grew || mn > m[mt][hh];
+            m[mt][hh] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[i] = exp2f(x[i] - ref); sum += x[i]; }
+            l[mt][hh] = l[mt][hh] * fac[mt][hh] + sum;
+            pf[mt][hh] = pack2<T>(x[0], x[1]);
+            pf[mt][2 + hh] = pack2<T>(x[2], x[3]);
+          }
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+              o[mt][i][0] *= fac[mt][0]; o[mt][i][1] *= fac[mt][0];
+              o[mt][i][2] *= fac[mt][1]; o[mt][i][3] *= fac[mt][1];
+            }
+        }
+        // A key that some rows may not see has p = 0 there, which a product with an infinity or NaN turns into NaN.
+        // Such values are looked for in the few stages where rows differ; there the keys then go one by one and rows
+        // that do not see a key keep what they had.
+        bool odd = false;
+        if (masked) {
+          for (int i = lane; i < KEYS * CPR; i += 32) {
+            const uint4 x = *reinterpret_cast<const uint4*>(smem + (vs_base - sbase) + i * 16);
+            odd = odd || any_nonfinite2<T>(x.x) || any_nonfinite2<T>(x.y) || any_nonfinite2<T>(x.z) || any_nonfinite2<T>(x.w);
+          }
+          odd = __any_sync(0xffffffffu, odd);
+        }
+        if (!odd) {
+#pragma unroll
+          for (int dn = 0; dn < D / 16; ++dn) {
+            uint32_t vf[4];
+            ldsm4_t(vf, vs_base + row_chunk<ROWB>(vrow, 2 * dn + vch));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16816<T>(o[mt][2 * dn], pf[mt], vf[0], vf[1]);
+              mma16816<T>(o[mt][2 * dn + 1], pf[mt], vf[2], vf[3]);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < KEYS; ++j) {
+            // this lane holds keys 2*(lane%4), +1 (registers 0, 1 of A; 0, 2 of B) and those + 8 (2, 3; 1, 3)
+            const uint32_t keep = (j & 7) / 2 == (lane & 3) ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+            const uint32_t k_lo = j < 8 ? keep : 0u, k_hi = j < 8 ? 0u : keep;
+#pragma unroll
+            for (int dn = 0; dn < D / 16; ++dn) {
+              uint32_t vf[4];
+              ldsm4_t(vf, vs_base + row_chunk<ROWB>(vrow, 2 * dn + vch));
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                const uint32_t a[4] = {pf[mt][0] & k_lo, pf[mt][1] & k_lo, pf[mt][2] & k_hi, pf[mt][3] & k_hi};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  float (&acc)[4] = o[mt][2 * dn + half];
+                  float next[4] = {acc[0], acc[1], acc[2], acc[3]};
+                  mma16816<T>(next, a, vf[2 * half] & k_lo, vf[2 * half + 1] & k_hi);
+                  if (key0 + j < lim[mt][0]) { acc[0] = next[0]; acc[1] = next[1]; }
+                  if (key0 + j < lim[mt][1]) { acc[2] = next[2]; acc[3] = next[3]; }
+                }
+              }
+            }
+          }
+        }
+      }
+      cp_async_wait<0>();
+      __syncthreads();                                                // the ring becomes the key groups' meeting place
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int r = rg * 16 * MT + mt * 16 + hh * 8 + (lane >> 2);
+          float sum = l[mt][hh];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          if ((lane & 3) == 0) s_ml[kg * R + r] = make_float2(m[mt][hh], sum);
+          float* dst = s_o + (kg * R + r) * D + 2 * (lane & 3);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[mt][i][2 * hh], o[mt][i][2 * hh + 1]);
+        }
+      }
+    } else {
+      // fp32: lane = key for the scores (32/KEYS groups of rows), lane = D/32 columns for the second product
+      constexpr int RPL = 16 * KEYS / 32;                             // score rows of a lane
+      constexpr int C = D / 32;                                       // output columns of a lane
+      float* s_p = reinterpret_cast<float*>(smem + S::P_OFF) + kg * (KEYS + 1) * 16;
+      float* s_f = s_p + KEYS * 16;
+      const int key_l = lane % KEYS, rbase = (lane / KEYS) * RPL;
+      float o[16][C], m[RPL], l[RPL];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int i = 0; i < C; ++i) o[r][i] = 0.0f;
+#pragma unroll
+      for (int r = 0; r < RPL; ++r) { m[r] = -INFINITY; l[r] = 0.0f; }
+      for (int t = 0; t < ntile; ++t) {
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();
+        issue(t + STAGES - 1);
+        const unsigned char* ks_base = smem + (ring - sbase) + (t % STAGES) * (2 * S::HALF_STAGE);
+        const unsigned char* vs_base = ks_base + S::HALF_STAGE;
+        const int key0 = (tile0 + t) * S::TILE + kg * KEYS;
+        if (key0 >= sq.ctx) continue;
+        float s[RPL];
+#pragma unroll
+        for (int r = 0; r < RPL; ++r) s[r] = 0.0f;
+#pragma unroll 4
+        for (int ch = 0; ch < CPR; ++ch) {
+          const float4 kv = *reinterpret_cast<const float4*>(ks_base + row_chunk<ROWB>(key_l, ch));
+#pragma unroll
+          for (int r = 0; r < RPL; ++r) {
+            const float4 qv = *reinterpret_cast<const float4*>(smem + S::Q_OFF + row_chunk<ROWB>(rbase + r, ch));
+            s[r] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[r]))));
+          }
+        }
+        const bool masked = key0 + KEYS > lim0;
+#pragma unroll
+        for (int r = 0; r < RPL; ++r) {
+          float x = s[r] * p.scale_log2;
+          if (masked && key0 + key_l >= limit(rbase + r)) x = -INFINITY;
+          float top = x;
+#pragma unroll
+          for (int w = KEYS / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          const float mn = fmaxf(m[r], top);
+          const float ref = mn == -INFINITY ? 0.0f : mn;
+          const float f = exp2f(m[r] - ref);
+          m[r] = mn;
+          x = exp2f(x - ref);
+          l[r] = l[r] * f + x;
+          s_p[key_l * 16 + rbase + r] = x;
+          if (key_l == 0) s_f[rbase + r] = f;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float f = s_f[r];
+#pragma unroll
+          for (int i = 0; i < C; ++i) o[r][i] *= f;
+        }
+        for (int j = 0; j < KEYS; ++j) {
+          float v[C];
+#pragma unroll
+          for (int i = 0; i < C; ++i) {
+            // the lane's columns are adjacent: C floats from column lane*C on
+            const int col = lane * C + i;
+            v[i] = *reinterpret_cast<const float*>(vs_base + row_chunk<ROWB>(j, col / 4) + (col % 4) * 4);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            // rows that do not see the key are left alone (0 * inf is not 0)
+            if (!masked || key0 + j < limit(r)) {
+              const float w = s_p[j * 16 + r];
+#pragma unroll
+              for (int i = 0; i < C; ++i) o[r][i] = fmaf(w, v[i], o[r][i]);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      cp_async_wait<0>();
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < RPL; ++r) {
+        float sum = l[r];
+#pragma unroll
+        for (int w = KEYS / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (key_l == 0) s_ml[kg * R + rbase + r] = make_float2(m[r], sum);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int i = 0; i < C; ++i) s_o[(kg * R + r) * D + lane * C + i] = o[r][i];
+    }
+    __syncthreads();
+
+    // --- join the key groups; write the output of a whole unit or the part of a cut one
+    for (int i = tid; i < rows * (D / 4); i += THREADS) {
+      const int r = i / (D / 4), c = i % (D / 4);
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) top = fmaxf(top, s_ml[k * R + r].x);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float l = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < KG; ++k) {
+        const float2 ml = s_ml[k * R + r];
+        const float f = exp2f(ml.x - ref);
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (k * R + r) * D + c * 4);
+        l = fmaf(ml.y, f, l);
+        acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+      }
+      if (whole) {
+        const int token = sq.first + (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;                // a row that sees no key gives zeros
+        T* dst = reinterpret_cast<T*>(p.out) + token * p.o_tok + h * p.o_head + c * 4;
+        if constexpr (kMma) {
+          uint2 v;
+          v.x = pack2<T>(acc.x * inv, acc.y * inv);
+          v.y = pack2<T>(acc.z * inv, acc.w * inv);
+          *reinterpret_cast<uint2*>(dst) = v;
+        } else {
+          *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
+        if (p.lse && c == 0) p.lse[(long long)token * p.Hq + h] = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+      } else {
+        *reinterpret_cast<float4*>(p.ws + ((long long)slot * R + r) * D + c * 4) = acc;
+        if (c == 0) reinterpret_cast<float2*>(p.ws + 2ll * p.grid * R * D)[(long long)slot * R + r] = make_float2(top, l);
+      }
+    }
+    __syncthreads();                                                  // before the ring and the queries are overwritten
+  }
+}
+
+// Joins the parts of the units that attn_kernel cut.  WPR warps (1 or 8) of the CTA's 8 share an output row.
+template <typename T, int D, int WPR>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int R) {
+  constexpr int RPC = 8 / WPR;
+  constexpr int C = D / 32;
+  __shared__ float s_acc[WPR > 1 ? 8 : 1][D];
+  __shared__ float2 s_ml[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  pdl_wait();
+  const long long row = (long long)blockIdx.x * RPC + warp / WPR;     // (token, head)
+  if (row >= (long long)p.T * p.Hq) return;                           // whole CTA when WPR is 8
+  const int token = (int)(row / p.Hq), h = (int)(row % p.Hq);
+  int b = token;
+  if (p.qstart) {
+    if (token >= p.qstart[p.B]) return;                               // behind the last sequence
+    int a = 0, e = p.B;                                               // last b with qstart[b] <= token
+    while (e - a > 1) {
+      const int mid = (a + e) >> 1;
+      if (p.qstart[mid] <= token) a = mid; else e = mid;
+    }
+    b = a;
+  } else if (b >= p.B) {
+    return;
+  }
+  const AttnSeq sq = attn_seq(p, b, R);
+  if (token < sq.first || token >= sq.first + sq.n) return;
+  const long long W = attn_work_before(p, p.B, R);
+  const int g = (int)(W < p.grid ? W : p.grid);
+  const int head = h / p.group, r_all = (token - sq.first) * p.group + h % p.group;
+  const int rt = r_all / R, r = r_all % R;
+  const long long u0 = attn_work_before(p, b, R) + (long long)(rt * p.Hkv + head) * sq.tiles;
+  const int c0 = attn_owner(W, g, u0), c1 = attn_owner(W, g, u0 + sq.tiles - 1);
+  if (c0 == c1) return;                                               // the unit was not cut
+  const float2* parts_ml = reinterpret_cast<const float2*>(p.ws + 2ll * p.grid * R * D);
+  float top = -INFINITY, l = 0.0f;
+  float acc[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) acc[i] = 0.0f;
+  // pass 1: the maximum of all parts; pass 2: the sums (independent loads)
+  for (int c = c0 + lane; c <= c1; c += 32) {
+    const int slot = 2 * c + (c == c0 ? 1 : 0);
+    top = fmaxf(top, parts_ml[(long long)slot * R + r].x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+  for (int c = c0 + warp % WPR; c <= c1; c += WPR) {
+    const int slot = 2 * c + (c == c0 ? 1 : 0);
+    const float2 ml = parts_ml[(long long)slot * R + r];
+    const float* src = p.ws + ((long long)slot * R + r) * D + lane * C;
+    const float f = exp2f(ml.x - ref);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int i = 0; i < C; ++i) acc[i] = fmaf(src[i], f, acc[i]);
+  }
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) s_acc[warp][lane * C + i] = acc[i];
+    if (lane == 0) s_ml[warp] = make_float2(0.0f, l);
+    __syncthreads();
+    if (warp != 0) return;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      l += s_ml[w].y;
+#pragma unroll
+      for (int i = 0; i < C; ++i) acc[i] += s_acc[w][lane * C + i];
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* dst = reinterpret_cast<T*>(p.out) + token * p.o_tok + h * p.o_head + lane * C;
+#pragma unroll
+  for (int i = 0; i < C; ++i) dst[i] = Elem<T>::from_float(acc[i] * inv);
+  if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace b200moe
