@@ -72,43 +72,56 @@ template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, 
 // launch, about as long as one CTA needs for them.
 constexpr long long kNoSplitSlots = 256;
 
+// What beginning a unit costs a CTA, in tiles of 64 keys, for the equal division of the work.
+constexpr int kUnitCost = 1;
+
 struct AttnPlan {
   int grid = 0, R = 0;
   int64_t ws_bytes = 0;
 };
 
+int sm_count(int dev, cudaError_t* err) {
+  static std::atomic<int> known[kMaxDevices];      // two threads that ask at once store the same number
+  int n = known[dev].load(std::memory_order_acquire);
+  if (n) return n;
+  *err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (*err == cudaSuccess) known[dev].store(n, std::memory_order_release);
+  return n;
+}
+
+// MINB CTAs fit an SM: they are what the grid holds, so that all parts of a call run at once.
 template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB> struct AttnVariant {
   using S = AttnShape<T, D, MT, RG, KG, STAGES>;
-  // CTAs that fill the device, kept per device; 0 = not asked yet.  Two threads that ask at once store the same number.
-  static int fill(int dev, cudaError_t* err) {
-    static std::atomic<int> known[kMaxDevices];
-    int n = known[dev].load(std::memory_order_acquire);
-    if (n) return n;
-    auto k = attn_kernel<T, D, MT, RG, KG, STAGES, MINB>;
-    int per_sm = 0, sms = 0;
-    *err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (*err == cudaSuccess) *err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, S::THREADS, S::SMEM);
-    if (*err == cudaSuccess) *err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (*err != cudaSuccess) return 0;
-    n = per_sm * sms;
-    if (n <= 0) { *err = cudaErrorLaunchOutOfResources; return 0; }
-    known[dev].store(n, std::memory_order_release);
-    return n;
+  static_assert(MINB * (S::SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
+
+  template <bool PAGE16> static cudaError_t start(const AttnParams& p, int dev, cudaStream_t s) {
+    static std::atomic<bool> ready[kMaxDevices];
+    auto k = attn_kernel<T, D, MT, RG, KG, STAGES, MINB, PAGE16>;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+      cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+      if (e != cudaSuccess) return e;
+      ready[dev].store(true, std::memory_order_release);
+    }
+    return launch(k, (unsigned)p.grid, S::THREADS, S::SMEM, s, p);
   }
   static cudaError_t run(AttnParams* p, int dev, AttnPlan* plan, cudaStream_t s, bool plan_only) {
     cudaError_t e = cudaSuccess;
-    plan->grid = fill(dev, &e);
+    plan->grid = MINB * sm_count(dev, &e);
     if (e != cudaSuccess) return e;
     plan->R = S::R;
     plan->ws_bytes = 2ll * plan->grid * S::R * (D + 2) * 4;
     if (plan_only) return cudaSuccess;
     p->grid = plan->grid;
     p->tile = S::TILE;
-    e = launch(attn_kernel<T, D, MT, RG, KG, STAGES, MINB>, (unsigned)plan->grid, S::THREADS, S::SMEM, s, *p);
+    p->unit_cost = kUnitCost;
+    e = p->block_size % 16 == 0 ? start<true>(*p, dev, s) : start<false>(*p, dev, s);
     if (e != cudaSuccess || !p->split) return e;
     const long long rows = (long long)p->T * p->Hq;
-    // Few rows are cut into many parts each: eight warps per row.  Many rows: one warp, or the launch grows.
-    if (rows <= 148 * 8) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R);
+    // As many warps per row as one CTA of eight on every SM allows: few rows are cut into many parts each, and a CTA
+    // that fits beside the attention kernel's has begun when that one ends.
+    if (rows <= 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R);
+    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), 256, 0, s, *p, S::R);
+    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), 256, 0, s, *p, S::R);
     return launch(attn_join_kernel<T, D, 1>, (unsigned)((rows + 7) / 8), 256, 0, s, *p, S::R);
   }
 };

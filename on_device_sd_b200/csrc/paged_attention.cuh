@@ -24,6 +24,8 @@
 // Roundings: scores, softmax, sums and accumulators are fp32; p is rounded to the cache's type for the second product
 // (the operand type of the tensor cores; the sum l uses the same unrounded p), outputs are rounded once.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "tma.cuh"
 
@@ -43,6 +45,7 @@ struct AttnParams {
   int B, T, Hq, Hkv, group, block_size, num_blocks, max_blocks;
   int split;                       // 0: units are not cut
   int tile;                        // keys of a tile
+  int unit_cost;                   // what beginning a unit costs, in tiles
   int grid;                        // CTAs of the attention kernel
 };
 
@@ -79,9 +82,9 @@ __device__ __forceinline__ void attn_report(const AttnParams& p, int b) {
   }
   if (bad) atomicOr(p.status, kDevBadLength);
 }
-__device__ __forceinline__ long long attn_work(const AttnParams& p, const AttnSeq& s) {
-  return (long long)s.row_tiles * p.Hkv * (p.split ? s.tiles : 1);
-}
+// A unit weighs its tiles and the cost of beginning it (the weight's first items stand for that).
+__device__ __forceinline__ int attn_weight(const AttnParams& p, const AttnSeq& s) { return p.split ? s.tiles + p.unit_cost : 1; }
+__device__ __forceinline__ long long attn_work(const AttnParams& p, const AttnSeq& s) { return (long long)s.row_tiles * p.Hkv * attn_weight(p, s); }
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -128,6 +131,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
   // a source size of zero fills the 16 bytes with zeros and reads nothing
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -136,6 +142,12 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 2^x, two units in the last place; results below 2^-126 become 0
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -177,31 +189,36 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES_> struct AttnSha
   static constexpr int ROWB = D * (int)sizeof(T);
   static constexpr int CPR = ROWB / 16;
   static constexpr int HALF_STAGE = KEYS * ROWB;   // K, then V
-  static constexpr int RING = KG * STAGES * 2 * HALF_STAGE;
-  static constexpr int JOIN = KG * R * D * 4;      // the key groups' o, in the ring's place
-  static constexpr int MAIN = RING > JOIN ? RING : JOIN;
-  static constexpr int Q_OFF = MAIN;
-  static constexpr int ML_OFF = Q_OFF + R * ROWB;
+  static constexpr int SLOT = 2 * HALF_STAGE;
+  static constexpr int RING = KG * STAGES * SLOT;
+  // At the end of a unit a key group leaves its o in JSLOTS slots of its ring; the others fetch the next unit meanwhile.
+  static constexpr int RPS = SLOT / (D * 4);       // rows of o in a slot
+  static constexpr int JSLOTS = (R + RPS - 1) / RPS;
+  static constexpr int AHEAD = STAGES - JSLOTS < STAGES - 1 ? STAGES - JSLOTS : STAGES - 1;
+  static constexpr int QB = R * ROWB;
+  static constexpr int Q_OFF = RING;               // two buffers
+  static constexpr int ML_OFF = Q_OFF + 2 * QB;
   static constexpr int P_OFF = ML_OFF + KG * R * 8;                        // fp32 only: p [KG][KEYS][16], factors [KG][16]
   static constexpr int SMEM = P_OFF + (sizeof(T) == 4 ? KG * (KEYS + 1) * 16 * 4 : 0);
+  static_assert(AHEAD >= 1, "room to fetch ahead");
 };
 
-template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB>
+// PAGE16: pages hold a multiple of 16 slots, so that the 16 keys of a stage lie in one page.
+template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, bool PAGE16>
 __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnParams p) {
   using S = AttnShape<T, D, MT, RG, KG, STAGES>;
   constexpr int R = S::R, ROWB = S::ROWB, CPR = S::CPR, KEYS = S::KEYS, THREADS = S::THREADS;
   constexpr bool kMma = sizeof(T) == 2;
-  static_assert(kMma ? KEYS == 16 : (MT == 1 && RG == 1 && KEYS <= 32), "shape");
-  extern __shared__ __align__(128) unsigned char smem[];
+  static_assert(kMma || (MT == 1 && RG == 1), "shape");
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kg = warp % KG, rg = warp / KG;
   const uint32_t sbase = smem_addr(smem);
-  const uint32_t ring = sbase + kg * (STAGES * 2 * S::HALF_STAGE);
-  float* s_o = reinterpret_cast<float*>(smem);
+  const uint32_t ring = sbase + kg * (STAGES * S::SLOT);
   float2* s_ml = reinterpret_cast<float2*>(smem + S::ML_OFF);
 
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();                   // after the wait: the join may then read this call's lengths before its own wait
   if (p.status)
     for (int b = blockIdx.x * THREADS + tid; b < p.B; b += gridDim.x * THREADS) attn_report(p, b);
   const long long W = attn_work_before(p, p.B, R);
@@ -209,84 +226,157 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   const int cta = blockIdx.x;
   if (cta >= g) return;
   long long lo = attn_lo(W, g, cta);
-  const long long my_lo = lo, hi = attn_lo(W, g, cta + 1);
+  const long long hi = attn_lo(W, g, cta + 1);
   long long seq_base;
-  int b = attn_find(p, lo, R, &seq_base);
+  int b_next = attn_find(p, lo, R, &seq_base);
   const T* kc = reinterpret_cast<const T*>(p.k);
   const T* vc = reinterpret_cast<const T*>(p.v);
 
-  while (lo < hi && b < p.B) {
-    const AttnSeq sq = attn_seq(p, b, R);
-    const long long seq_work = attn_work(p, sq);
-    if (lo >= seq_base + seq_work) { seq_base += seq_work; ++b; continue; }
-    const int weight = p.split ? sq.tiles : 1;
-    const int unit = (int)((lo - seq_base) / weight);
-    const int skip = (int)((lo - seq_base) % weight);                 // tiles of this unit that other CTAs took
-    const long long left = hi - lo;
-    const int tile0 = skip;
-    const int ntile = p.split ? (int)(left < weight - skip ? left : weight - skip) : sq.tiles;
-    const bool whole = !p.split || (skip == 0 && ntile == weight);
-    const int slot = 2 * cta + (lo == my_lo && skip > 0 ? 0 : 1);
-    lo += p.split ? ntile : 1;
-    const int rt = unit / p.Hkv, head = unit % p.Hkv;
-    const int row0 = rt * R, rows = min(R, sq.n * p.group - row0);    // rows of the sequence: token-major, then head of the group
+  // --- this CTA's units, one after the other
+  struct Unit {
+    int first, ctx, n;             // the sequence: query row, keys, new tokens
+    int head, row0, rows;          // rows row0 .. row0 + rows - 1 of the sequence: token-major, then head of the group
+    int tile0, ntile, part;        // part: where a cut unit's result goes, -1 for a whole one
+    const int* table;
+  };
+  auto next_unit = [&](Unit* u) -> bool {
+    while (lo < hi && b_next < p.B) {
+      const AttnSeq sq = attn_seq(p, b_next, R);
+      const long long seq_work = attn_work(p, sq);
+      if (lo >= seq_base + seq_work) { seq_base += seq_work; ++b_next; continue; }
+      const int weight = attn_weight(p, sq);
+      const int unit = (int)((lo - seq_base) / weight), skip = (int)((lo - seq_base) % weight);
+      const int take = (int)min(hi - lo, (long long)(weight - skip));
+      lo += take;
+      int t0 = 0, t1 = sq.tiles;
+      if (p.split) {
+        t0 = max(skip - p.unit_cost, 0);
+        t1 = skip + take - p.unit_cost;
+        if (t1 <= t0) continue;    // only the part that stands for the beginning
+      }
+      u->first = sq.first; u->ctx = sq.ctx; u->n = sq.n;
+      u->head = unit % p.Hkv;
+      u->row0 = unit / p.Hkv * R;
+      u->rows = min(R, sq.n * p.group - u->row0);
+      u->tile0 = t0; u->ntile = t1 - t0;
+      // a part that begins inside a unit is this CTA's first, one that ends inside a unit its last
+      u->part = t1 - t0 == sq.tiles ? -1 : 2 * cta + (t0 > 0 ? 0 : 1);
+      u->table = p.tables + (long long)b_next * p.table_stride;
+      return true;
+    }
+    return false;
+  };
 
-    // --- loads of the cache: the 16 lanes of a row fetch its chunks; lane j < KEYS knows where key j of the stage lies
-    const int* table = p.tables + (long long)b * p.table_stride;
-    const T* kh = kc + head * p.c_head;
-    const T* vh = vc + head * p.c_head;
-    int page_next = 0;
-    auto lookup = [&](int t) {                                        // page of this lane's key of tile t (one stage ahead)
-      const int key = (tile0 + t) * S::TILE + kg * KEYS + (lane % KEYS);
-      page_next = (t < ntile && key < sq.ctx) ? __ldg(table + key / p.block_size) : -1;
-    };
-    auto issue = [&](int t) {
-      if (t < ntile) {
-        const int key = (tile0 + t) * S::TILE + kg * KEYS + (lane % KEYS);
-        const bool in = key < sq.ctx;
-        const bool ok = in && page_next >= 0 && page_next < p.num_blocks;
-        if (in && !ok && p.status) atomicOr(p.status, kDevBadPage);
-        const long long off = ok ? page_next * p.c_block + (long long)(key % p.block_size) * p.c_slot : -1;
-        const uint32_t dst = ring + (t % STAGES) * (2 * S::HALF_STAGE);
-        const int pt = rg * 32 + lane;
-        constexpr int STEP = 32 * RG;
-#pragma unroll
-        for (int i = 0; i < (KEYS * CPR + STEP - 1) / STEP; ++i) {
+  // --- loads: a key group fills slot after slot of its ring with 16 keys and values
+  constexpr int STEP = 32 * RG;                                       // lanes that fill a stage
+  constexpr int COPIES = (KEYS * CPR + STEP - 1) / STEP;
+  const int pt = rg * 32 + lane;
+  int page_next = 0;
+  auto lookup = [&](const Unit& u, int t) {                           // page of this lane's key of tile t (one stage ahead)
+    const int key = (u.tile0 + t) * S::TILE + kg * KEYS + (PAGE16 ? 0 : lane % KEYS);
+    page_next = (t < u.ntile && key < u.ctx) ? __ldg(u.table + key / p.block_size) : -1;
+  };
+  auto issue = [&](const Unit& u, int t, int slot_at) {
+    if (t < u.ntile) {
+      const int key0 = (u.tile0 + t) * S::TILE + kg * KEYS;
+      const uint32_t dst = ring + slot_at * S::SLOT;
+      const T* kh = kc + u.head * p.c_head;
+      const T* vh = vc + u.head * p.c_head;
+      const int key = key0 + (PAGE16 ? 0 : lane % KEYS);              // the key whose page this lane looked up
+      const bool in = key < u.ctx;
+      const bool ok = in && page_next >= 0 && page_next < p.num_blocks;
+      if (in && !ok && p.status) atomicOr(p.status, kDevBadPage);
+      const long long off = ok ? page_next * p.c_block + (long long)(key % p.block_size) * p.c_slot : 0;
+      if constexpr (PAGE16) {
+        // a lane's rows are STEP/CPR apart at one chunk (or, in rows longer than a step, its chunks STEP apart)
+        constexpr int DROW = CPR <= STEP ? STEP / CPR : 0;
+        const long long e = off + (pt / CPR) * p.c_slot + (pt % CPR) * (16 / (int)sizeof(T));
+        const T* ks = kh + e;
+        const T* vs = vh + e;
+        auto place = [&](int i, int* row, int* ch, long long* delta) {
           const int idx = pt + i * STEP;
-          const int row = idx / CPR, ch = idx % CPR;
-          const long long o = __shfl_sync(0xffffffffu, off, row % KEYS);
-          if (KEYS * CPR % STEP == 0 || idx < KEYS * CPR) {
-            const long long e = (o < 0 ? 0 : o) + ch * (16 / (int)sizeof(T));
+          *row = idx / CPR;
+          *ch = idx % CPR;
+          *delta = DROW ? (long long)(i * DROW) * p.c_slot : (long long)(*row - pt / CPR) * p.c_slot + (*ch - pt % CPR) * (16 / (int)sizeof(T));
+        };
+        int row, ch;
+        long long delta;
+        if (ok && key0 + KEYS <= u.ctx && KEYS * CPR % STEP == 0) {
+#pragma unroll
+          for (int i = 0; i < COPIES; ++i) {
+            place(i, &row, &ch, &delta);
             const uint32_t d = dst + row_chunk<ROWB>(row, ch);
-            cp_async16(d, kh + e, o >= 0);
-            cp_async16(d + S::HALF_STAGE, vh + e, o >= 0);
+            cp_async16(d, ks + delta);
+            cp_async16(d + S::HALF_STAGE, vs + delta);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < COPIES; ++i) {
+            place(i, &row, &ch, &delta);
+            if (row < KEYS) {
+              const bool there = ok && key0 + row < u.ctx;
+              const uint32_t d = dst + row_chunk<ROWB>(row, ch);
+              cp_async16(d, there ? ks + delta : kc, there);
+              cp_async16(d + S::HALF_STAGE, there ? vs + delta : vc, there);
+            }
           }
         }
-        lookup(t + 1);
-      }
-      cp_async_commit();
-    };
-    lookup(0);
+      } else {
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) issue(t);
-
-    // --- queries
+        for (int i = 0; i < COPIES; ++i) {
+          const int idx = pt + i * STEP;
+          const int row = idx / CPR, ch = idx % CPR;
+          const long long o = __shfl_sync(0xffffffffu, ok ? off : -1, row % KEYS);
+          if (KEYS * CPR % STEP == 0 || idx < KEYS * CPR) {
+            const long long e = o + ch * (16 / (int)sizeof(T));
+            const uint32_t d = dst + row_chunk<ROWB>(row, ch);
+            cp_async16(d, o < 0 ? kc : kh + e, o >= 0);
+            cp_async16(d + S::HALF_STAGE, o < 0 ? vc : vh + e, o >= 0);
+          }
+        }
+      }
+      lookup(u, t + 1);
+    }
+    cp_async_commit();
+  };
+  auto slot_after = [](int at, int d) { return at + d >= STAGES ? at + d - STAGES : at + d; };   // d <= STAGES
+  // the queries of a unit (into one of two buffers) and its first stages
+  auto begin = [&](const Unit& u, int at, int qbuf) {
+    lookup(u, 0);
     for (int i = tid; i < R * CPR; i += THREADS) {
       const int r = i / CPR, ch = i % CPR;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int token = sq.first + (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
-        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + token * p.q_tok + h * p.q_head + ch * (16 / (int)sizeof(T)));
-      }
-      *reinterpret_cast<uint4*>(smem + S::Q_OFF + row_chunk<ROWB>(r, ch)) = x;
+      const int token = u.first + (u.row0 + r) / p.group, h = u.head * p.group + (u.row0 + r) % p.group;
+      const T* src = reinterpret_cast<const T*>(p.q) + token * p.q_tok + h * p.q_head + ch * (16 / (int)sizeof(T));
+      cp_async16(sbase + S::Q_OFF + qbuf * S::QB + row_chunk<ROWB>(r, ch), r < u.rows ? src : reinterpret_cast<const T*>(p.q), r < u.rows);
     }
-    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < S::AHEAD; ++t) issue(u, t, slot_after(at, t));
+  };
+  // where row r, column c of key group k's o lies while the groups meet: `at` is the ring slot of the next stage
+  auto o_place = [&](int k, int r, int c, int at) -> float* {
+    const int slot = slot_after(at, S::AHEAD + r / S::RPS);
+    const int unit32 = (c >> 3) ^ (r & (D / 8 < 8 ? D / 8 - 1 : 7));  // 32-byte units permuted: the 8 rows of a fragment in different banks
+    return reinterpret_cast<float*>(smem + (k * STAGES + slot) * S::SLOT + (r % S::RPS) * (D * 4) + unit32 * 32 + (c & 7) * 4);
+  };
 
-    const int lim0 = sq.ctx - sq.n + 1 + row0 / p.group;              // keys that the first (and least seeing) row sees
-    auto limit = [&](int r) { return sq.ctx - sq.n + 1 + (row0 + min(r, rows - 1)) / p.group; };
+  Unit u;
+  bool more = next_unit(&u);
+  int at = 0, qbuf = 0;                                               // ring slot of the stage in hand, buffer of the queries
+  if (more) begin(u, at, qbuf);
+  while (more) {
+#pragma unroll
+    for (int t = S::AHEAD; t < STAGES - 1; ++t) issue(u, t, slot_after(at, t));
+    cp_async_wait<STAGES - 2>();                                      // the queries have come with the first stage
+    __syncthreads();
+    const int rows = u.rows, row0 = u.row0;
+    const int lim0 = u.ctx - u.n + 1 + row0 / p.group;                // keys that the first (and least seeing) row sees
+    auto limit = [&](int r) { return u.ctx - u.n + 1 + (row0 + min(r, rows - 1)) / p.group; };
+    Unit nu;
 
     if constexpr (kMma) {
-      // rows lane/4 and lane/4 + 8 of each 16-row tile, columns 2*(lane%4), +1 of each 8-column tile
+      // rows lane/4 and lane/4 + 8 of each 16-row tile, columns 2*(lane%4), +1 of each 8-column tile.  Row tiles go to the
+      // row groups in turn; tiles without a row are left out.
+      const int mts = min(MT, ((rows + 15) / 16 - rg + RG - 1) / RG);
       float o[MT][D / 8][4];
       float m[MT][2], l[MT][2];
       int lim[MT][2];
@@ -297,45 +387,40 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           m[mt][hh] = -INFINITY; l[mt][hh] = 0.0f;
-          lim[mt][hh] = limit(rg * 16 * MT + mt * 16 + hh * 8 + (lane >> 2));
+          lim[mt][hh] = limit((mt * RG + rg) * 16 + hh * 8 + (lane >> 2));
         }
       }
-      const uint32_t qbase = sbase + S::Q_OFF;
-      const int qrow = rg * 16 * MT + (lane & 7) + ((lane >> 3) & 1) * 8, qch = lane >> 4;
-      const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
-      const int vrow = (lane & 7) + ((lane >> 3) & 1) * 8, vch = lane >> 4;
+      // Fragment addresses: a step of 16 columns is two chunks, and an exclusive or with it keeps the permutation.
+      const uint32_t q_off = sbase + S::Q_OFF + qbuf * S::QB + row_chunk<ROWB>(rg * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
+      const uint32_t k_off = row_chunk<ROWB>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+      const uint32_t v_off = S::HALF_STAGE + row_chunk<ROWB>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
       constexpr bool kQRegs = MT == 1 && D <= 128;                    // else the registers are needed for o
       uint32_t qf[kQRegs ? D / 16 : 1][4];
       if constexpr (kQRegs) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) ldsm4(qf[ks], qbase + row_chunk<ROWB>(qrow, 2 * ks + qch));
+        for (int ks = 0; ks < D / 16; ++ks) ldsm4(qf[ks], q_off ^ (ks << 5));
       }
 
-      for (int t = 0; t < ntile; ++t) {
-        cp_async_wait<STAGES - 2>();
-        if constexpr (RG > 1) bar_sync(1 + kg, 32 * RG); else __syncwarp();
-        issue(t + STAGES - 1);
-        const uint32_t ks_base = ring + (t % STAGES) * (2 * S::HALF_STAGE), vs_base = ks_base + S::HALF_STAGE;
-        const int key0 = (tile0 + t) * S::TILE + kg * KEYS;
-        if (key0 >= sq.ctx) continue;                                 // nothing of the last tile in this group
-
-        float s[MT][2][4];
+      // One stage (16 keys) for the first M row tiles of this warp
+      auto stage = [&](auto tiles, uint32_t base, int key0) {
+        constexpr int M = decltype(tiles)::value;
+        float s[M][2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < M; ++mt)
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t kf[4];
-          ldsm4(kf, ks_base + row_chunk<ROWB>(krow, 2 * ks + kch));
+          ldsm4(kf, (base + k_off) ^ (ks << 5));
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
+          for (int mt = 0; mt < M; ++mt) {
             if constexpr (kQRegs) {
               mma16816<T>(s[mt][0], qf[ks], kf[0], kf[1]);
               mma16816<T>(s[mt][1], qf[ks], kf[2], kf[3]);
             } else {
               uint32_t a[4];
-              ldsm4(a, qbase + row_chunk<ROWB>(qrow + mt * 16, 2 * ks + qch));
+              ldsm4(a, (q_off ^ (ks << 5)) + mt * (RG * 16 * ROWB));
               mma16816<T>(s[mt][0], a, kf[0], kf[1]);
               mma16816<T>(s[mt][1], a, kf[2], kf[3]);
             }
@@ -343,44 +428,61 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         }
 
         const bool masked = key0 + KEYS > lim0;
-        uint32_t pf[MT][4];
-        bool grew = false;
-        float fac[MT][2];
+        if (masked) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+          for (int mt = 0; mt < M; ++mt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int key = key0 + (i >> 2) * 8 + 2 * (lane & 3) + (i & 1);
+              if (key >= lim[mt][(i >> 1) & 1]) s[mt][i >> 2][i & 3] = -INFINITY;
+            }
+        }
+        // m is the reference that p is taken against: a maximum of the row that is renewed only when the row has
+        // outgrown it by 2^8, so that o is seldom rescaled.  p stays below 2^8 (in range of fp16), l and o are
+        // relative to the same reference.
+        bool grew = false;
+        float top[M][2];
+#pragma unroll
+        for (int mt = 0; mt < M; ++mt) {
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int key = key0 + (i >> 1) * 8 + 2 * (lane & 3) + (i & 1);
-              x[i] = s[mt][i >> 1][2 * hh + (i & 1)] * p.scale_log2;
-              if (masked && key >= lim[mt][hh]) x[i] = -INFINITY;
-            }
-            float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float mn = fmaxf(m[mt][hh], top);
-            const float ref = mn == -INFINITY ? 0.0f : mn;            // a row that has seen nothing yet
-            fac[mt][hh] = exp2f(m[mt][hh] - ref);
-            grew = grew || mn > m[mt][hh];
-            m[mt][hh] = mn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { x[i] = exp2f(x[i] - ref); sum += x[i]; }
-            l[mt][hh] = l[mt][hh] * fac[mt][hh] + sum;
-            pf[mt][hh] = pack2<T>(x[0], x[1]);
-            pf[mt][2 + hh] = pack2<T>(x[2], x[3]);
+            float x = fmaxf(fmaxf(s[mt][0][2 * hh], s[mt][0][2 * hh + 1]), fmaxf(s[mt][1][2 * hh], s[mt][1][2 * hh + 1]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            top[mt][hh] = x * p.scale_log2;
+            grew = grew || top[mt][hh] > m[mt][hh] + 8.0f;
           }
         }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int mt = 0; mt < M; ++mt) {
+            float fac[2];
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              const bool renew = top[mt][hh] > m[mt][hh] + 8.0f;
+              fac[hh] = renew ? ex2(m[mt][hh] - top[mt][hh]) : 1.0f;
+              if (renew) m[mt][hh] = top[mt][hh];
+              l[mt][hh] *= fac[hh];
+            }
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) {
-              o[mt][i][0] *= fac[mt][0]; o[mt][i][1] *= fac[mt][0];
-              o[mt][i][2] *= fac[mt][1]; o[mt][i][3] *= fac[mt][1];
+              o[mt][i][0] *= fac[0]; o[mt][i][1] *= fac[0];
+              o[mt][i][2] *= fac[1]; o[mt][i][3] *= fac[1];
             }
+          }
+        }
+        uint32_t pf[M][4];
+#pragma unroll
+        for (int mt = 0; mt < M; ++mt) {
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const float ref = m[mt][hh] == -INFINITY ? 0.0f : m[mt][hh];      // a row that has seen nothing yet
+            const float x0 = ex2(fmaf(s[mt][0][2 * hh], p.scale_log2, -ref)), x1 = ex2(fmaf(s[mt][0][2 * hh + 1], p.scale_log2, -ref));
+            const float x2 = ex2(fmaf(s[mt][1][2 * hh], p.scale_log2, -ref)), x3 = ex2(fmaf(s[mt][1][2 * hh + 1], p.scale_log2, -ref));
+            l[mt][hh] += (x0 + x1) + (x2 + x3);
+            pf[mt][hh] = pack2<T>(x0, x1);
+            pf[mt][2 + hh] = pack2<T>(x2, x3);
+          }
         }
         // A key that some rows may not see has p = 0 there, which a product with an infinity or NaN turns into NaN.
         // Such values are looked for in the few stages where rows differ; there the keys then go one by one and rows
@@ -388,7 +490,7 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         bool odd = false;
         if (masked) {
           for (int i = lane; i < KEYS * CPR; i += 32) {
-            const uint4 x = *reinterpret_cast<const uint4*>(smem + (vs_base - sbase) + i * 16);
+            const uint4 x = *reinterpret_cast<const uint4*>(smem + (base - sbase) + S::HALF_STAGE + i * 16);
             odd = odd || any_nonfinite2<T>(x.x) || any_nonfinite2<T>(x.y) || any_nonfinite2<T>(x.z) || any_nonfinite2<T>(x.w);
           }
           odd = __any_sync(0xffffffffu, odd);
@@ -397,9 +499,9 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
 #pragma unroll
           for (int dn = 0; dn < D / 16; ++dn) {
             uint32_t vf[4];
-            ldsm4_t(vf, vs_base + row_chunk<ROWB>(vrow, 2 * dn + vch));
+            ldsm4_t(vf, (base + v_off) ^ (dn << 5));
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int mt = 0; mt < M; ++mt) {
               mma16816<T>(o[mt][2 * dn], pf[mt], vf[0], vf[1]);
               mma16816<T>(o[mt][2 * dn + 1], pf[mt], vf[2], vf[3]);
             }
@@ -413,9 +515,9 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
 #pragma unroll
             for (int dn = 0; dn < D / 16; ++dn) {
               uint32_t vf[4];
-              ldsm4_t(vf, vs_base + row_chunk<ROWB>(vrow, 2 * dn + vch));
+              ldsm4_t(vf, (base + v_off) ^ (dn << 5));
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
+              for (int mt = 0; mt < M; ++mt) {
                 const uint32_t a[4] = {pf[mt][0] & k_lo, pf[mt][1] & k_lo, pf[mt][2] & k_hi, pf[mt][3] & k_hi};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -429,21 +531,38 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
             }
           }
         }
+      };
+
+      for (int t = 0; t < u.ntile; ++t) {
+        cp_async_wait<STAGES - 2>();
+        if constexpr (RG > 1) bar_sync(1 + kg, 32 * RG); else __syncwarp();
+        issue(u, t + STAGES - 1, slot_after(at, STAGES - 1));
+        const uint32_t base = ring + at * S::SLOT;
+        at = slot_after(at, 1);
+        const int key0 = (u.tile0 + t) * S::TILE + kg * KEYS;
+        if (key0 >= u.ctx) continue;                                  // nothing of the last tile in this group
+        if constexpr (MT == 2) {
+          if (mts == 2) stage(std::integral_constant<int, 2>{}, base, key0);
+          else if (mts == 1) stage(std::integral_constant<int, 1>{}, base, key0);
+        } else {
+          if (RG == 1 || mts == 1) stage(std::integral_constant<int, 1>{}, base, key0);
+        }
       }
-      cp_async_wait<0>();
-      __syncthreads();                                                // the ring becomes the key groups' meeting place
+      if constexpr (RG > 1) bar_sync(1 + kg, 32 * RG); else __syncwarp();   // the ring is free
+      more = next_unit(&nu);
+      if (more) begin(nu, at, qbuf ^ 1);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          const int r = rg * 16 * MT + mt * 16 + hh * 8 + (lane >> 2);
+          const int r = (mt * RG + rg) * 16 + hh * 8 + (lane >> 2);
           float sum = l[mt][hh];
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
           if ((lane & 3) == 0) s_ml[kg * R + r] = make_float2(m[mt][hh], sum);
-          float* dst = s_o + (kg * R + r) * D + 2 * (lane & 3);
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[mt][i][2 * hh], o[mt][i][2 * hh + 1]);
+          for (int i = 0; i < D / 8; ++i)
+            *reinterpret_cast<float2*>(o_place(kg, r, i * 8 + 2 * (lane & 3), at)) = make_float2(o[mt][i][2 * hh], o[mt][i][2 * hh + 1]);
         }
       }
     } else {
@@ -460,14 +579,16 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         for (int i = 0; i < C; ++i) o[r][i] = 0.0f;
 #pragma unroll
       for (int r = 0; r < RPL; ++r) { m[r] = -INFINITY; l[r] = 0.0f; }
-      for (int t = 0; t < ntile; ++t) {
+      const unsigned char* s_q = smem + S::Q_OFF + qbuf * S::QB;
+      for (int t = 0; t < u.ntile; ++t) {
         cp_async_wait<STAGES - 2>();
         __syncwarp();
-        issue(t + STAGES - 1);
-        const unsigned char* ks_base = smem + (ring - sbase) + (t % STAGES) * (2 * S::HALF_STAGE);
+        issue(u, t + STAGES - 1, slot_after(at, STAGES - 1));
+        const unsigned char* ks_base = smem + (ring - sbase) + at * S::SLOT;
+        at = slot_after(at, 1);
         const unsigned char* vs_base = ks_base + S::HALF_STAGE;
-        const int key0 = (tile0 + t) * S::TILE + kg * KEYS;
-        if (key0 >= sq.ctx) continue;
+        const int key0 = (u.tile0 + t) * S::TILE + kg * KEYS;
+        if (key0 >= u.ctx) continue;
         float s[RPL];
 #pragma unroll
         for (int r = 0; r < RPL; ++r) s[r] = 0.0f;
@@ -476,23 +597,23 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
           const float4 kv = *reinterpret_cast<const float4*>(ks_base + row_chunk<ROWB>(key_l, ch));
 #pragma unroll
           for (int r = 0; r < RPL; ++r) {
-            const float4 qv = *reinterpret_cast<const float4*>(smem + S::Q_OFF + row_chunk<ROWB>(rbase + r, ch));
+            const float4 qv = *reinterpret_cast<const float4*>(s_q + row_chunk<ROWB>(rbase + r, ch));
             s[r] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[r]))));
           }
         }
         const bool masked = key0 + KEYS > lim0;
 #pragma unroll
         for (int r = 0; r < RPL; ++r) {
-          float x = s[r] * p.scale_log2;
+          float x = s[r];
           if (masked && key0 + key_l >= limit(rbase + r)) x = -INFINITY;
-          float top = x;
+          float top = x * p.scale_log2;
 #pragma unroll
           for (int w = KEYS / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
           const float mn = fmaxf(m[r], top);
           const float ref = mn == -INFINITY ? 0.0f : mn;
-          const float f = exp2f(m[r] - ref);
+          const float f = ex2(m[r] - ref);
           m[r] = mn;
-          x = exp2f(x - ref);
+          x = ex2(fmaf(x, p.scale_log2, -ref));
           l[r] = l[r] * f + x;
           s_p[key_l * 16 + rbase + r] = x;
           if (key_l == 0) s_f[rbase + r] = f;
@@ -524,8 +645,8 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         }
         __syncwarp();
       }
-      cp_async_wait<0>();
-      __syncthreads();
+      more = next_unit(&nu);
+      if (more) begin(nu, at, qbuf ^ 1);
 #pragma unroll
       for (int r = 0; r < RPL; ++r) {
         float sum = l[r];
@@ -536,7 +657,7 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
 #pragma unroll
       for (int r = 0; r < 16; ++r)
 #pragma unroll
-        for (int i = 0; i < C; ++i) s_o[(kg * R + r) * D + lane * C + i] = o[r][i];
+        for (int i = 0; i < C; ++i) *o_place(kg, r, lane * C + i, at) = o[r][i];
     }
     __syncthreads();
 
@@ -552,13 +673,13 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
 #pragma unroll
       for (int k = 0; k < KG; ++k) {
         const float2 ml = s_ml[k * R + r];
-        const float f = exp2f(ml.x - ref);
-        const float4 x = *reinterpret_cast<const float4*>(s_o + (k * R + r) * D + c * 4);
+        const float f = ex2(ml.x - ref);
+        const float4 x = *reinterpret_cast<const float4*>(o_place(k, r, c * 4, at));
         l = fmaf(ml.y, f, l);
         acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
       }
-      if (whole) {
-        const int token = sq.first + (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
+      if (u.part < 0) {
+        const int token = u.first + (row0 + r) / p.group, h = u.head * p.group + (row0 + r) % p.group;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;                // a row that sees no key gives zeros
         T* dst = reinterpret_cast<T*>(p.out) + token * p.o_tok + h * p.o_head + c * 4;
         if constexpr (kMma) {
@@ -571,15 +692,20 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         }
         if (p.lse && c == 0) p.lse[(long long)token * p.Hq + h] = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
       } else {
-        *reinterpret_cast<float4*>(p.ws + ((long long)slot * R + r) * D + c * 4) = acc;
-        if (c == 0) reinterpret_cast<float2*>(p.ws + 2ll * p.grid * R * D)[(long long)slot * R + r] = make_float2(top, l);
+        *reinterpret_cast<float4*>(p.ws + ((long long)u.part * R + r) * D + c * 4) = acc;
+        if (c == 0) reinterpret_cast<float2*>(p.ws + 2ll * p.grid * R * D)[(long long)u.part * R + r] = make_float2(top, l);
       }
     }
-    __syncthreads();                                                  // before the ring and the queries are overwritten
+    qbuf ^= 1;
+    u = nu;
+    __syncthreads();                                                  // before the slots that held o are filled again
   }
 }
 
-// Joins the parts of the units that attn_kernel cut.  WPR warps (1 or 8) of the CTA's 8 share an output row.
+// Joins the parts of the units that attn_kernel cut.  WPR warps (1, 2, 4 or 8) of the CTA's 8 share an output row.  What
+// depends on the lengths alone is found out before the wait for attn_kernel: that kernel lets this one start only after
+// its own wait, so the lengths are complete.  No warp leaves before the wait - the next kernel takes the end of this
+// grid for the end of both.
 template <typename T, int D, int WPR>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int R) {
   constexpr int RPC = 8 / WPR;
@@ -588,70 +714,75 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int 
   __shared__ float2 s_ml[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
-  pdl_wait();
   const long long row = (long long)blockIdx.x * RPC + warp / WPR;     // (token, head)
-  if (row >= (long long)p.T * p.Hq) return;                           // whole CTA when WPR is 8
   const int token = (int)(row / p.Hq), h = (int)(row % p.Hq);
+  bool cut = token < p.T;
   int b = token;
-  if (p.qstart) {
-    if (token >= p.qstart[p.B]) return;                               // behind the last sequence
+  if (cut && p.qstart) {
     int a = 0, e = p.B;                                               // last b with qstart[b] <= token
     while (e - a > 1) {
       const int mid = (a + e) >> 1;
       if (p.qstart[mid] <= token) a = mid; else e = mid;
     }
     b = a;
-  } else if (b >= p.B) {
-    return;
   }
-  const AttnSeq sq = attn_seq(p, b, R);
-  if (token < sq.first || token >= sq.first + sq.n) return;
-  const long long W = attn_work_before(p, p.B, R);
-  const int g = (int)(W < p.grid ? W : p.grid);
-  const int head = h / p.group, r_all = (token - sq.first) * p.group + h % p.group;
-  const int rt = r_all / R, r = r_all % R;
-  const long long u0 = attn_work_before(p, b, R) + (long long)(rt * p.Hkv + head) * sq.tiles;
-  const int c0 = attn_owner(W, g, u0), c1 = attn_owner(W, g, u0 + sq.tiles - 1);
-  if (c0 == c1) return;                                               // the unit was not cut
-  const float2* parts_ml = reinterpret_cast<const float2*>(p.ws + 2ll * p.grid * R * D);
+  cut = cut && b < p.B;
+  int c0 = 0, c1 = 0, r = 0;
+  if (cut) {
+    const AttnSeq sq = attn_seq(p, b, R);
+    cut = token >= sq.first && token < sq.first + sq.n;
+    if (cut) {
+      const long long W = attn_work_before(p, p.B, R);
+      const int g = (int)(W < p.grid ? W : p.grid);
+      const int head = h / p.group, r_all = (token - sq.first) * p.group + h % p.group;
+      r = r_all % R;
+      const long long u0 = attn_work_before(p, b, R) + (long long)(r_all / R * p.Hkv + head) * attn_weight(p, sq) + p.unit_cost;
+      c0 = attn_owner(W, g, u0);
+      c1 = attn_owner(W, g, u0 + sq.tiles - 1);
+      cut = c0 != c1;                                                 // else one CTA has written the output
+    }
+  }
+  pdl_wait();
   float top = -INFINITY, l = 0.0f;
   float acc[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) acc[i] = 0.0f;
-  // pass 1: the maximum of all parts; pass 2: the sums (independent loads)
-  for (int c = c0 + lane; c <= c1; c += 32) {
-    const int slot = 2 * c + (c == c0 ? 1 : 0);
-    top = fmaxf(top, parts_ml[(long long)slot * R + r].x);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float ref = top == -INFINITY ? 0.0f : top;
+  if (cut) {
+    const float2* parts_ml = reinterpret_cast<const float2*>(p.ws + 2ll * p.grid * R * D);
 #pragma unroll 4
-  for (int c = c0 + warp % WPR; c <= c1; c += WPR) {
-    const int slot = 2 * c + (c == c0 ? 1 : 0);
-    const float2 ml = parts_ml[(long long)slot * R + r];
-    const float* src = p.ws + ((long long)slot * R + r) * D + lane * C;
-    const float f = exp2f(ml.x - ref);
-    l = fmaf(ml.y, f, l);
+    for (int c = c0 + warp % WPR; c <= c1; c += WPR) {
+      const long long part = (long long)(2 * c + (c == c0 ? 1 : 0)) * R + r;
+      const float2 ml = parts_ml[part];
+      const float* src = p.ws + part * D + lane * C;
+      const float mn = fmaxf(top, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+      const float f0 = ex2(top - ref), f1 = ex2(ml.x - ref);
+      l = fmaf(l, f0, ml.y * f1);
 #pragma unroll
-    for (int i = 0; i < C; ++i) acc[i] = fmaf(src[i], f, acc[i]);
+      for (int i = 0; i < C; ++i) acc[i] = fmaf(acc[i], f0, src[i] * f1);
+      top = mn;
+    }
   }
   if constexpr (WPR > 1) {
 #pragma unroll
     for (int i = 0; i < C; ++i) s_acc[warp][lane * C + i] = acc[i];
-    if (lane == 0) s_ml[warp] = make_float2(0.0f, l);
+    if (lane == 0) s_ml[warp] = make_float2(top, l);
     __syncthreads();
-    if (warp != 0) return;
+    if (warp % WPR != 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) top = fmaxf(top, s_ml[warp + w].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < C; ++i) acc[i] = 0.0f;
 #pragma unroll
     for (int w = 0; w < WPR; ++w) {
-      l += s_ml[w].y;
+      const float f = ex2(s_ml[warp + w].x - ref);
+      l = fmaf(s_ml[warp + w].y, f, l);
 #pragma unroll
-      for (int i = 0; i < C; ++i) acc[i] += s_acc[w][lane * C + i];
+      for (int i = 0; i < C; ++i) acc[i] = fmaf(s_acc[warp + w][lane * C + i], f, acc[i]);
     }
   }
+  if (!cut) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   T* dst = reinterpret_cast<T*>(p.out) + token * p.o_tok + h * p.o_head + lane * C;
 #pragma unroll
