@@ -73,7 +73,13 @@ template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, 
 constexpr long long kNoSplitSlots = 256;
 
 // What beginning a unit costs a CTA, in tiles of 64 keys, for the equal division of the work.
-constexpr int kUnitCost = 1;
+#ifndef UC
+#define UC 3
+#endif
+#ifndef RB
+#define RB 3
+#endif
+constexpr int kUnitCost = UC;
 
 struct AttnPlan {
   int grid = 0, R = 0;
@@ -90,13 +96,13 @@ int sm_count(int dev, cudaError_t* err) {
 }
 
 // MINB CTAs fit an SM: they are what the grid holds, so that all parts of a call run at once.
-template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB> struct AttnVariant {
+template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int REGB = MINB> struct AttnVariant {
   using S = AttnShape<T, D, MT, RG, KG, STAGES>;
   static_assert(MINB * (S::SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
 
   template <bool PAGE16> static cudaError_t start(const AttnParams& p, int dev, cudaStream_t s) {
     static std::atomic<bool> ready[kMaxDevices];
-    auto k = attn_kernel<T, D, MT, RG, KG, STAGES, MINB, PAGE16>;
+    auto k = attn_kernel<T, D, MT, RG, KG, STAGES, REGB, PAGE16>;
     if (!ready[dev].load(std::memory_order_acquire)) {
       cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
       if (e != cudaSuccess) return e;
@@ -147,9 +153,13 @@ template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int rows, 
         if (rows <= 32) return AttnVariant<T, 64, 2, 1, 4, 4, 3>::run(p, dev, plan, s, po);
         return AttnVariant<T, 64, 2, 2, 4, 5, 2>::run(p, dev, plan, s, po);
       case 128:
-        if (rows <= 16) return AttnVariant<T, 128, 1, 1, 4, 3, 2>::run(p, dev, plan, s, po);
+        if (rows <= 16) return AttnVariant<T, 128, 1, 1, 4, 3, 2, RB>::run(p, dev, plan, s, po);
         if (rows <= 32) return AttnVariant<T, 128, 2, 1, 4, 3, 2>::run(p, dev, plan, s, po);
+#ifdef R64
+        return AttnVariant<T, 128, 1, 4, 4, 6, 1>::run(p, dev, plan, s, po);
+#else
         return AttnVariant<T, 128, 2, 2, 4, 6, 1>::run(p, dev, plan, s, po);
+#endif
       default:
         if (rows <= 16) return AttnVariant<T, 256, 1, 1, 4, 3, 1>::run(p, dev, plan, s, po);
         return AttnVariant<T, 256, 1, 2, 4, 3, 1>::run(p, dev, plan, s, po);

@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
       const uint32_t q_off = sbase + S::Q_OFF + qbuf * S::QB + row_chunk<ROWB>(rg * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
       const uint32_t k_off = row_chunk<ROWB>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
       const uint32_t v_off = S::HALF_STAGE + row_chunk<ROWB>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
-      constexpr bool kQRegs = MT == 1 && D <= 128;                    // else the registers are needed for o
+      constexpr bool kQRegs = MT == 1 && RG == 1 && D <= 128;         // else the registers are needed for o
       uint32_t qf[kQRegs ? D / 16 : 1][4];
       if constexpr (kQRegs) {
 #pragma unroll
