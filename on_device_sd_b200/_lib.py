@@ -12,6 +12,7 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libb200moe.so"
+STEP_PATH = PKG / "_step.so"
 
 OK, E_ARG, E_CUDA, E_STATE, E_DEVICE, E_UNSUPPORTED = 0, 1, 2, 3, 4, 5
 F32, F16, BF16 = 0, 1, 2
@@ -108,6 +109,7 @@ PROTOTYPES = {
 }
 
 _lib = None
+_step = None
 
 
 class B200MoEError(RuntimeError):
@@ -137,6 +139,19 @@ def load() -> ctypes.CDLL:
         raise ImportError(f"{LIB_PATH} has ABI version {lib.b200moe_abi_version()}, this binding expects {ABI_VERSION}; rebuild it")
     _lib = lib
     return lib
+
+
+def load_step():
+    """The tensor entry points of the step operators (csrc/bindings.cpp), built beside libb200moe.so and linked to it."""
+    global _step
+    if _step is None:
+        if not STEP_PATH.exists():
+            raise ImportError(f"{STEP_PATH} is missing: build it with `python -m on_device_sd_b200.build`. There is no fallback path.")
+        load()
+        import torch  # noqa: F401  (the libraries that _step.so is linked to)
+        from importlib import import_module
+        _step = import_module("on_device_sd_b200._step")
+    return _step
 
 
 def check(ctx, code: int) -> None:

@@ -1,8 +1,9 @@
-"""Builds libb200moe.so in-tree with nvcc for sm_100a (no other architecture is supported).
+"""Builds libb200moe.so in-tree with nvcc for sm_100a (no other architecture is supported), and _step.so, the
+tensor entry points of the step operators (csrc/bindings.cpp), with the host compiler against the installed torch.
 
     python -m on_device_sd_b200.build [--force] [--verbose]
 
-The shared library lands next to this file so that it travels with the source tree; nothing
+The shared libraries land next to this file so that they travel with the source tree; nothing
 is installed into site-packages and no JIT cache is used.
 """
 from __future__ import annotations
@@ -16,11 +17,12 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libb200moe.so"
+STEP = PKG / "_step.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr", "--extended-lambda",
 ]
 
@@ -53,19 +55,56 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found; libb200moe.so cannot be built")
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not _stale():
-        return LIB
-    cmd = [nvcc_path(), *NVCC_FLAGS, *_defines(), "-I", str(PKG.parent / "include"), "-o", str(LIB)]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += [str(s) for s in _sources()]
-    cmd += ["-lcuda"] if (CSRC / "ffn_umma.cuh").exists() else []
+def _build_step(force: bool, verbose: bool) -> None:
+    src = CSRC / "bindings.cpp"
+    deps = (src, PKG.parent / "include" / "b200moe.h", Path(__file__))
+    if not force and STEP.exists() and all(p.stat().st_mtime <= STEP.stat().st_mtime for p in deps):
+        return
+    import sysconfig
+
+    import torch
+    tdir = Path(torch.__file__).parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(tdir / "include"), "-isystem", str(cuda / "include"),
+           str(src), "-o", str(STEP), "-L", str(tdir / "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda",
+           "-L", str(PKG), "-lb200moe", "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
     if res.returncode != 0:
+        raise RuntimeError("the host compiler failed building _step.so:\n" + res.stderr[-4000:])
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    if not force and not _stale():
+        _build_step(False, verbose)
+        return LIB
+    import tempfile
+    from concurrent.futures import ThreadPoolExecutor
+    nvcc = nvcc_path()
+    flags = [*NVCC_FLAGS, *_defines(), "-I", str(PKG.parent / "include"), *(["-Xptxas", "-v"] if verbose else [])]
+    with tempfile.TemporaryDirectory() as tmp:
+        def compile_one(src: Path):
+            obj = Path(tmp) / (src.stem + ".o")
+            return obj, subprocess.run([nvcc, *flags, "-c", str(src), "-o", str(obj)], capture_output=True, text=True)
+
+        with ThreadPoolExecutor() as pool:
+            done = list(pool.map(compile_one, _sources()))
+        for _, res in done:
+            if verbose or res.returncode != 0:
+                sys.stderr.write(res.stdout + res.stderr)
+            if res.returncode != 0:
+                raise RuntimeError("nvcc failed building libb200moe.so:\n" + res.stderr[-4000:])
+        cmd = [nvcc, *NVCC_FLAGS, "-shared", "-o", str(LIB), *[str(o) for o, _ in done]]
+        cmd += ["-lcuda"] if (CSRC / "ffn_umma.cuh").exists() else []
+        res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+    if res.returncode != 0:
         raise RuntimeError("nvcc failed building libb200moe.so:\n" + res.stderr[-4000:])
+    _build_step(True, verbose)
     return LIB
 
 

@@ -26,8 +26,7 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream(device: torch.device) -> int:
-    """The handle of the device's current stream, without the Stream object torch.cuda.current_stream makes (2 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _need_cuda(t: torch.Tensor, name: str, device: torch.device, dtype: Optional[torch.dtype] = None) -> None:
