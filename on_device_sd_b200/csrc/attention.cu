@@ -209,7 +209,9 @@ extern "C" int b200moe_store_kv(const b200moe_store_kv_args* a, void* stream) {
                              a->o_token_stride, a->o_head_stride, a->cache_block_stride, a->cache_slot_stride, a->cache_head_stride};
   for (int64_t s : strides)
     if (odd_stride(s, dt)) return b200moe_fail_global(B200MOE_E_ARG, "%s: strides must be multiples of 16 bytes", who);
-  if ((int64_t)a->num_tokens * (a->num_heads + 2ll * a->num_kv_heads) > (1ll << 36)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: too many heads x tokens", who);
+  // heads are numbered in 32 bits, up to the end of the last CTA
+  if ((int64_t)a->num_tokens * ((has_q ? a->num_heads : 0) + 2ll * a->num_kv_heads) > (1ll << 31))
+    return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: more than 2^31 tokens x heads", who);
   int dev;
   if (int rc = current_device(who, &dev)) return rc;
   StoreKvParams p = {};

@@ -57,10 +57,10 @@ __global__ void __launch_bounds__(kStoreThreads) store_kv_kernel(const StoreKvPa
   pdl_trigger();
   pdl_wait();
   const int heads = p.Hq + 2 * p.Hkv;
-  const int groups = (heads + kHeads - 1) / kHeads;
-  const long long item = ((long long)blockIdx.x * kStoreThreads + threadIdx.x) / L;
+  const unsigned groups = (unsigned)(heads + kHeads - 1) / kHeads;
+  const unsigned item = blockIdx.x * (unsigned)(kStoreThreads / L) + threadIdx.x / L;   // below 2^32, as the caller checks
   const int sub = threadIdx.x % L;
-  const bool live = item < (long long)p.T * groups;   // whole lane groups; idle ones still take part in the shuffles
+  const bool live = item < p.T * groups;              // whole lane groups; idle ones still take part in the shuffles
   const int t = live ? (int)(item / groups) : 0;
   const int h0 = live ? (int)(item % groups) * kHeads : heads;
 
@@ -77,7 +77,14 @@ __global__ void __launch_bounds__(kStoreThreads) store_kv_kernel(const StoreKvPa
     atomicOr(p.status, (bad_pos ? kDevBadPosition : 0) | (bad_slot ? kDevBadSlot : 0));
   const bool keep = slot >= 0 && !bad_slot && !bad_pos;
   long long cache_off = 0;
-  if (keep) cache_off = (slot / p.block_size) * p.c_block + (slot % p.block_size) * p.c_slot;
+  if (keep) {
+    if (slot <= 0xffffffffll) {                       // a 64-bit division costs as much as the rest of a head
+      const unsigned s32 = (unsigned)slot, blk = s32 / (unsigned)p.block_size;
+      cache_off = blk * p.c_block + (s32 - blk * p.block_size) * p.c_slot;
+    } else {
+      cache_off = (slot / p.block_size) * p.c_block + (slot % p.block_size) * p.c_slot;
+    }
+  }
 
   float c[8], s[8];
 #pragma unroll

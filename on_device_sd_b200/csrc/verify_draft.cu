@@ -16,14 +16,20 @@ template <typename T> cudaError_t launch_verify(const VerifyParams& p, cudaStrea
   const bool vec = (p.V * sizeof(T)) % 16 == 0 && (p.target_stride * sizeof(T)) % 16 == 0 && ((uintptr_t)p.target & 15u) == 0 &&
                    (!p.draft || ((p.draft_stride * sizeof(T)) % 16 == 0 && ((uintptr_t)p.draft & 15u) == 0));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.B * kVerifyCluster);
+  // eight CTAs per sequence until four on every SM (what the registers allow) are taken, fewer for larger batches
+  unsigned cluster = kVerifyMaxCluster;
+  while (cluster > 1 && (long long)p.B * cluster > 4 * 148) cluster /= 2;
+  cfg.gridDim = dim3((unsigned)p.B * cluster);
   cfg.blockDim = dim3(kVerifyThreads);
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return vec ? cudaLaunchKernelEx(&cfg, verify_draft_kernel<T, true>, p) : cudaLaunchKernelEx(&cfg, verify_draft_kernel<T, false>, p);
 }
 

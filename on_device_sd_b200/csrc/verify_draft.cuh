@@ -5,10 +5,11 @@
 // A draw with the given number u takes the first i with r_0 + ... + r_i > u * (r_0 + ... + r_{V-1}).
 //
 // Neighbouring tokens of a large vocabulary are closer in the running sum than fp32 resolves, so differences and
-// sums are taken in 64 bits.  What bounds it is HBM (one or two rows of the vocabulary per sequence) and, for one
-// sequence, the chain of dependent loads start -> token -> probability.  A cluster of eight CTAs shares a row: each
-// warp sums one contiguous piece, all sums meet in every CTA's shared memory over the cluster, and the warp whose piece
-// holds the draw reads it again (from L2) to find the token.  One launch, no workspace, no atomics.
+// sums are taken in 64 bits.  What bounds it is HBM for large batches (one or two rows of the vocabulary per sequence)
+// and, for small ones, a chain of dependent loads: start -> token -> probability -> row -> the place in the row.
+// A cluster of CTAs shares a sequence: each warp sums one contiguous piece of the row, all sums meet in every CTA's
+// shared memory over the cluster, and the CTA whose piece holds the draw reads it again (from L2), all its warps side by
+// side, to find the token.  One launch, no workspace, no atomics in global memory.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -29,9 +30,10 @@ struct VerifyParams {
   int B, V, max_draft, num_draft, target_rows;
 };
 
-constexpr int kVerifyCluster = 8;
-constexpr int kVerifyThreads = 512;
-constexpr int kVerifyPieces = kVerifyCluster * (kVerifyThreads / 32);
+constexpr int kVerifyMaxCluster = 8;
+constexpr int kVerifyThreads = 256;
+constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyPieces = kVerifyMaxCluster * kVerifyWarps;        // at most; 64
 
 __device__ __forceinline__ double warp_scan_incl(double v) {
   const int lane = threadIdx.x & 31;
@@ -71,15 +73,40 @@ __device__ __forceinline__ void load_rest(const T* p, const T* q, int skip, int 
   for (int k = 0; k < E; ++k) r[k] = r[k] > 0.0 && i + k != skip ? r[k] : 0.0;   // a NaN counts as nothing
 }
 
+// The first of up to 2 x 32 sums (two per lane, in index order) with which the running sum passes `goal`, and the sum
+// before it; without one, the last that is positive.  By a whole warp; -1 when none is positive.
+struct Found { int at; bool passed; double before, total; };
+__device__ __forceinline__ Found find_sum(double s0, double s1, double base, double u, bool relative, double goal) {
+  const int lane = threadIdx.x & 31;
+  const double own = s0 + s1, incl = warp_scan_incl(own);
+  Found f;
+  f.total = __shfl_sync(0xffffffffu, incl, 31);
+  if (relative) goal = u * f.total;
+  const double run = base + (incl - own);
+  const bool h0 = s0 > 0.0 && run + s0 > goal, h1 = s1 > 0.0 && run + s0 + s1 > goal;
+  const unsigned has = __ballot_sync(0xffffffffu, h0 || h1);
+  f.passed = has != 0;
+  if (has) {
+    const int src = __ffs(has) - 1;
+    f.at = __shfl_sync(0xffffffffu, h0 ? 2 * lane : 2 * lane + 1, src);
+    f.before = __shfl_sync(0xffffffffu, h0 ? run : run + s0, src);
+  } else {
+    f.at = __reduce_max_sync(0xffffffffu, s1 > 0.0 ? 2 * lane + 1 : (s0 > 0.0 ? 2 * lane : -1));
+    f.before = 0.0;
+  }
+  return f;
+}
+
 template <typename T, bool VEC>
-__global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerifyThreads) verify_draft_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_draft_kernel(const VerifyParams p) {
   namespace cg = cooperative_groups;
   constexpr int E = 16 / (int)sizeof(T);
-  constexpr int WARPS = kVerifyThreads / 32;
+  constexpr int UNIT = 32 * E;                                        // a warp's elements per step
   __shared__ double s_sum[2][kVerifyPieces];
+  __shared__ double s_part[kVerifyWarps];
   __shared__ int s_first;
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), b = blockIdx.x / kVerifyCluster;
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / C;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
   pdl_wait();
@@ -107,11 +134,12 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
   __syncthreads();
   for (int j = threadIdx.x; j < n; j += kVerifyThreads) {
     const long long x = p.tokens[base + j];
+    const float uj = p.accept[base + j];
     bool take = false;
     if (x >= 0 && x < p.V) {
       const double pj = (double)Elem<T>::to_float(target[j * p.target_stride + x]);
       const double qj = draft ? (double)Elem<T>::to_float(draft[((long long)base + j) * p.draft_stride + x]) : 1.0;
-      take = pj > (double)p.accept[base + j] * qj;                    // exact in 64 bits; a NaN refuses
+      take = pj > (double)uj * qj;                                    // exact in 64 bits; a NaN refuses
     } else if (p.status && rank == 0) {
       atomicOr(p.status, kDevBadToken);
     }
@@ -131,15 +159,14 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
   long long gone = -1;
   if (taken < n && !draft) gone = p.tokens[base + taken];
   int skip = gone >= 0 && gone < p.V ? (int)gone : -1;
-  const int piece = rank * WARPS + warp;
-  const int unit = 32 * E;                                            // a warp's elements per step
-  const int per = ((p.V + kVerifyPieces - 1) / kVerifyPieces + E - 1) / E * E;
+  const int pieces = C * kVerifyWarps, piece = rank * kVerifyWarps + warp;
+  const int per = ((p.V + pieces - 1) / pieces + E - 1) / E * E;
   const int lo = (int)min((long long)piece * per, (long long)p.V), hi = min(lo + per, p.V);
 
   for (int round = 0; round < 2; ++round) {
     double sum = 0.0;
-#pragma unroll 2
-    for (int i = lo + lane * E; i < hi; i += unit) {
+#pragma unroll 4
+    for (int i = lo + lane * E; i < hi; i += UNIT) {
       double r[E];
       load_rest<T, E, VEC>(row, less, skip, i, hi, r);
 #pragma unroll
@@ -147,16 +174,12 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
     }
     sum = warp_sum(sum);
     if (round == 0) cluster.barrier_wait();
-    if (lane < kVerifyCluster) *cluster.map_shared_rank(&s_sum[round][piece], lane) = sum;
+    if (lane < C) *cluster.map_shared_rank(&s_sum[round][piece], lane) = sum;
     cluster.sync();
-    // piece sums in index order: lane holds pieces 4*lane .. +3
-    constexpr int PL = kVerifyPieces / 32;
-    double mine[PL], own = 0.0;
-#pragma unroll
-    for (int k = 0; k < PL; ++k) { mine[k] = s_sum[round][lane * PL + k]; own += mine[k]; }
-    const double incl = warp_scan_incl(own);
-    const double total = __shfl_sync(0xffffffffu, incl, 31);
-    if (!(total > 0.0)) {                                             // the same in every CTA
+    // every warp finds the piece that holds the draw, or the last with anything in it
+    const bool l0 = 2 * lane < pieces, l1 = 2 * lane + 1 < pieces;
+    const Found f = find_sum(l0 ? s_sum[round][2 * lane] : 0.0, l1 ? s_sum[round][2 * lane + 1] : 0.0, 0.0, (double)u, true, 0.0);
+    if (!(f.total > 0.0)) {                                           // the same in every CTA
       if (round == 0 && (less || skip >= 0)) { less = nullptr; skip = -1; continue; }   // nothing is left of p - q: draw from p
       if (rank == 0 && threadIdx.x == 0) {
         out[taken] = -1;
@@ -164,37 +187,34 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
       }
       return;
     }
-    const double goal = (double)u * total;
-    // the first piece whose running sum passes the goal, else the last that holds anything
-    double run = incl - own, before = 0.0;
-    int first = kVerifyPieces, last = -1;
+    if (f.at / kVerifyWarps != rank) return;
+    // this CTA owns it: each warp takes a share of the piece
+    const double goal = (double)u * f.total;
+    const int plo = (int)min((long long)f.at * per, (long long)p.V), phi = min(plo + per, p.V);
+    const int share = ((phi - plo + kVerifyWarps - 1) / kVerifyWarps + E - 1) / E * E;
+    const int slo = min(plo + warp * share, phi), shi = min(slo + share, phi);
+    sum = 0.0;
+    for (int i = slo + lane * E; i < shi; i += UNIT) {
+      double r[E];
+      load_rest<T, E, VEC>(row, less, skip, i, shi, r);
 #pragma unroll
-    for (int k = 0; k < PL; ++k) {
-      if (mine[k] > 0.0) {
-        last = lane * PL + k;
-        if (first == kVerifyPieces && run + mine[k] > goal) { first = lane * PL + k; before = run; }
-      }
-      run += mine[k];
+      for (int k = 0; k < E; ++k) sum += r[k];
     }
-    const unsigned has = __ballot_sync(0xffffffffu, first < kVerifyPieces);
-    int target_piece;
-    if (has) {
-      const int src = __ffs(has) - 1;
-      target_piece = __shfl_sync(0xffffffffu, first, src);
-      before = __shfl_sync(0xffffffffu, before, src);
-    } else {
-      target_piece = __reduce_max_sync(0xffffffffu, last);
-      before = 0.0;
-    }
-    if (target_piece != piece) return;
-    // this warp's piece holds the draw
+    sum = warp_sum(sum);
+    if (lane == 0) s_part[warp] = sum;
+    __syncthreads();
+    const Found w = find_sum(lane < kVerifyWarps / 2 ? s_part[2 * lane] : 0.0, lane < kVerifyWarps / 2 ? s_part[2 * lane + 1] : 0.0, f.before, 0.0, false,
+                             f.passed ? goal : (double)INFINITY);
+    if (w.at != warp) return;
+    double before = w.before;
+    const bool want = f.passed && w.passed;                           // else the last token with any weight
     int found = -1, last_pos = -1;
-    for (int i0 = lo; i0 < hi && found < 0; i0 += unit) {
+    for (int i0 = slo; i0 < shi && found < 0; i0 += UNIT) {
       const int i = i0 + lane * E;
       double r[E], s = 0.0;
 #pragma unroll
       for (int k = 0; k < E; ++k) r[k] = 0.0;
-      if (i < hi) load_rest<T, E, VEC>(row, less, skip, i, hi, r);
+      if (i < shi) load_rest<T, E, VEC>(row, less, skip, i, shi, r);
 #pragma unroll
       for (int k = 0; k < E; ++k) s += r[k];
       const double inc = warp_scan_incl(s);
@@ -205,7 +225,7 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
         if (r[k] > 0.0) {
           at += r[k];
           pos = i + k;
-          if (has && here < 0 && at > goal) here = i + k;
+          if (want && here < 0 && at > goal) here = i + k;
         }
       }
       const unsigned hit = __ballot_sync(0xffffffffu, here >= 0);
