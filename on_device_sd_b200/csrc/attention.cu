@@ -47,14 +47,17 @@ cudaError_t launch(void (*kernel)(Params...), unsigned grid, unsigned threads, s
 // ---------------------------------------------------------------------------------------------
 // b200moe_store_kv
 // ---------------------------------------------------------------------------------------------
+#ifndef KH
+#define KH 4
+#endif
 template <typename T, int D> cudaError_t launch_store(const StoreKvParams& p, cudaStream_t s) {
   constexpr int L = D / 16;
   const int heads = p.Hq + 2 * p.Hkv;
   // One head per lane group until that fills the GPU about twice (148 SMs x 2048 threads), four from there on.
   const bool wide = (long long)p.T * heads * L >= 2ll * 148 * 2048;
-  const long long groups = (long long)p.T * (wide ? (heads + 3) / 4 : heads);
+  const long long groups = (long long)p.T * (wide ? (heads + KH - 1) / KH : heads);
   const unsigned grid = (unsigned)((groups * L + kStoreThreads - 1) / kStoreThreads);
-  return wide ? launch(store_kv_kernel<T, D, 4>, grid, kStoreThreads, 0, s, p) : launch(store_kv_kernel<T, D, 1>, grid, kStoreThreads, 0, s, p);
+  return wide ? launch(store_kv_kernel<T, D, KH>, grid, kStoreThreads, 0, s, p) : launch(store_kv_kernel<T, D, 1>, grid, kStoreThreads, 0, s, p);
 }
 template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, cudaStream_t s) {
   switch (D) {

@@ -45,32 +45,43 @@ __device__ __forceinline__ double warp_scan_incl(double v) {
   return v;
 }
 
-// E consecutive elements as doubles; VEC: one 16-byte load
-template <typename T, int E, bool VEC> __device__ __forceinline__ void load_probs(const T* p, int i, int end, double (&f)[E]) {
+// E consecutive elements; VEC: one 16-byte load, else what lies before `end`
+template <typename T, int E, bool VEC> __device__ __forceinline__ void load_probs(const T* p, int i, int end, float (&f)[E]) {
   if constexpr (VEC) {
     static_assert(E * sizeof(T) == 16, "one vector");
     const uint4 raw = ldg_cached(p + i);
     const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int k = 0; k < E; ++k) f[k] = (double)Elem<T>::to_float(e[k]);
+    for (int k = 0; k < E; ++k) f[k] = Elem<T>::to_float(e[k]);
   } else {
 #pragma unroll
-    for (int k = 0; k < E; ++k) f[k] = i + k < end ? (double)Elem<T>::to_float(p[i + k]) : 0.0;
+    for (int k = 0; k < E; ++k) f[k] = i + k < end ? Elem<T>::to_float(p[i + k]) : 0.0f;
   }
 }
 
-// r_i of the draw: what is left of p after the draft's share; `skip` is a token that has none
+// r_i of the draw: what is left of p after the draft's share, never negative; `skip` is a token that has none.  Which
+// elements count is decided in fp32, where the comparison is exact and a NaN counts as nothing; the rest is in 64 bits.
 template <typename T, int E, bool VEC>
 __device__ __forceinline__ void load_rest(const T* p, const T* q, int skip, int i, int end, double (&r)[E]) {
-  load_probs<T, E, VEC>(p, i, end, r);
+  float f[E];
+  load_probs<T, E, VEC>(p, i, end, f);
   if (q) {
-    double s[E];
+    float s[E];
     load_probs<T, E, VEC>(q, i, end, s);
 #pragma unroll
-    for (int k = 0; k < E; ++k) r[k] -= s[k];
-  }
+    for (int k = 0; k < E; ++k) {
+      const bool left = f[k] > s[k] && f[k] > 0.0f;
+      r[k] = (double)(left ? f[k] : 0.0f) - (double)(left ? s[k] : 0.0f);
+    }
+  } else {
 #pragma unroll
-  for (int k = 0; k < E; ++k) r[k] = r[k] > 0.0 && i + k != skip ? r[k] : 0.0;   // a NaN counts as nothing
+    for (int k = 0; k < E; ++k) r[k] = (double)fmaxf(f[k], 0.0f);
+  }
+  if ((unsigned)(skip - i) < (unsigned)E) {
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+      if (i + k == skip) r[k] = 0.0;
+  }
 }
 
 // The first of up to 2 x 32 sums (two per lane, in index order) with which the running sum passes `goal`, and the sum
