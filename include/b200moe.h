@@ -324,9 +324,9 @@ int b200moe_store_kv(const b200moe_store_kv_args* args, void* stream);
  * (B200MOE_DEV_BAD_PAGE; that sequence's output is not to be used); lengths that do not fit the tensors are cut, and
  * spans that do not are skipped (B200MOE_DEV_BAD_LENGTH).
  * max_query_len: the longest span; longer ones are computed correctly, but read the cache more often.
- * workspace: as many bytes as b200moe_paged_attention_workspace gives for the same dtype, heads and max_query_len
- * and for max_context = max_blocks_per_seq * block_size on this device; it need not be cleared and must not be
- * shared by calls that may overlap.  NULL: sequences are not cut along the cache (slower for long ones). */
+ * workspace: as many bytes as b200moe_paged_attention_workspace gives for the same numbers on the same device (0 for
+ * short contexts; max_query_len is 1 without query_start); it need not be cleared and must not be shared by calls that
+ * may overlap.  NULL: sequences are not cut along the cache (slower for long ones). */
 typedef struct b200moe_paged_attention_args {
   const void* query;                    /* [num_tokens, num_heads, head_dim]                        */
   const void *k_cache, *v_cache;
@@ -345,8 +345,8 @@ typedef struct b200moe_paged_attention_args {
   int32_t reserved;
 } b200moe_paged_attention_args;
 int b200moe_paged_attention(const b200moe_paged_attention_args* args, void* stream);
-int b200moe_paged_attention_workspace(int dtype, int num_heads, int num_kv_heads, int head_dim, int max_query_len, int64_t max_context,
-                                      int64_t* bytes_out);
+int b200moe_paged_attention_workspace(int dtype, int num_seqs, int num_heads, int num_kv_heads, int head_dim, int max_query_len,
+                                      int max_blocks_per_seq, int block_size, int64_t* bytes_out);
 
 /* Verifies drafted tokens against the target's probabilities by rejection sampling with given random numbers, for all
  * sequences at once (the engine's _execute_accept is a host loop with a threshold rule,
@@ -356,7 +356,7 @@ int b200moe_paged_attention_workspace(int dtype, int num_heads, int num_kv_heads
  *   at the first refusal a token is drawn from max(p_j - q_j, 0) (draft_probs NULL: p_j without x; p_j if nothing is
  *   left), after n accepted tokens from p_n: the first i with r_0 + ... + r_i > sample_uniform[b] * (r_0 + ... + r_V-1),
  *   the last i with r_i > 0 if there is none.
- * Comparisons, differences and sums are in 64 bits; rows need not be normalised; negative values and NaN count as 0.
+ * Comparisons, differences and sums are in 64 bits; rows need not be normalised; an r that is negative or NaN counts as 0.
  *   tokens_out int64 [num_seqs, max_draft_len + 1]: the accepted tokens, the drawn one, then -1;  accepted_out [num_seqs].
  * A token outside the vocabulary is refused (B200MOE_DEV_BAD_TOKEN).  Where a row holds nothing to draw from, the drawn
  * token is -1 (B200MOE_DEV_BAD_PROBS).  A sequence whose numbers do not fit the tensors gets a row of -1 and 0

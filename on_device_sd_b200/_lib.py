@@ -99,7 +99,7 @@ PROTOTYPES = {
     "b200moe_unpack_int4": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "b200moe_store_kv": (c_int, [POINTER(StoreKvArgs), c_void_p]),
     "b200moe_paged_attention": (c_int, [POINTER(PagedAttentionArgs), c_void_p]),
-    "b200moe_paged_attention_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int64, POINTER(c_int64)]),
+    "b200moe_paged_attention_workspace": (c_int, [c_int] * 8 + [POINTER(c_int64)]),
     "b200moe_verify_draft": (c_int, [POINTER(VerifyDraftArgs), c_void_p]),
     "b200moe_profile": (c_int, [c_void_p, c_int]),
     "b200moe_profile_read": (c_int, [c_void_p, c_void_p, c_void_p]),

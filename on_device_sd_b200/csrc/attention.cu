@@ -47,17 +47,14 @@ cudaError_t launch(void (*kernel)(Params...), unsigned grid, unsigned threads, s
 // ---------------------------------------------------------------------------------------------
 // b200moe_store_kv
 // ---------------------------------------------------------------------------------------------
-#ifndef KH
-#define KH 4
-#endif
 template <typename T, int D> cudaError_t launch_store(const StoreKvParams& p, cudaStream_t s) {
   constexpr int L = D / 16;
   const int heads = p.Hq + 2 * p.Hkv;
   // One head per lane group until that fills the GPU about twice (148 SMs x 2048 threads), four from there on.
   const bool wide = (long long)p.T * heads * L >= 2ll * 148 * 2048;
-  const long long groups = (long long)p.T * (wide ? (heads + KH - 1) / KH : heads);
+  const long long groups = (long long)p.T * (wide ? (heads + 3) / 4 : heads);
   const unsigned grid = (unsigned)((groups * L + kStoreThreads - 1) / kStoreThreads);
-  return wide ? launch(store_kv_kernel<T, D, KH>, grid, kStoreThreads, 0, s, p) : launch(store_kv_kernel<T, D, 1>, grid, kStoreThreads, 0, s, p);
+  return wide ? launch(store_kv_kernel<T, D, 4>, grid, kStoreThreads, 0, s, p) : launch(store_kv_kernel<T, D, 1>, grid, kStoreThreads, 0, s, p);
 }
 template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, cudaStream_t s) {
   switch (D) {
@@ -71,22 +68,19 @@ template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, 
 // ---------------------------------------------------------------------------------------------
 // b200moe_paged_attention
 // ---------------------------------------------------------------------------------------------
-// Up to this many cache slots per sequence (pages x page size) a unit is not cut: joining its parts would cost a second
-// launch, about as long as one CTA needs for them.
-constexpr long long kNoSplitSlots = 256;
-
-// What beginning a unit costs a CTA, in tiles of 64 keys, for the equal division of the work.
-#ifndef UC
-#define UC 3
-#endif
-#ifndef RB
-#define RB 3
-#endif
-constexpr int kUnitCost = UC;
+// Whether a call's units are cut along the cache over the whole grid, from what the host knows: B sequences of at most
+// max_blocks * block_size slots.  Uncut, a unit belongs to one CTA, which takes about 1 us for a tile (4 us in fp32) when it
+// has the time to itself; cut, a second kernel joins the parts, about 2 us.  16-bit types, 4 kv heads, us uncut / cut:
+// one sequence of 33 slots 5.5 / 7.2, of 200 8.6 / 7.2 (so 4 tiles, half of them used on average, go uncut); 16 of up to
+// 200 7.7 / 9.8.  Units that just fill the GPU once gain longer: 64 sequences of up to 500 slots 14.6 / 16.5, of 1000
+// 24.1 / 21.6; with 8 kv heads, more units than fit at once, 25.5 / 23.2 at 500.
+constexpr int kUncutTiles = 4, kUncutTilesFull = 8, kUncutTilesF32 = 1;
+// What beginning a unit costs a CTA, in tiles of 64 keys, for the equal division of the work.  (32 spans over 100..2500
+// tokens: 55.2 us at 0, 48.0 at 1, 44.2 at 2, 42.8 at 3; equal lengths do not care.)
+constexpr int kUnitCost = 3;
 
 struct AttnPlan {
-  int grid = 0, R = 0;
-  int64_t ws_bytes = 0;
+  int64_t ws_bytes = 0;            // 0: units are not cut
 };
 
 int sm_count(int dev, cudaError_t* err) {
@@ -103,7 +97,7 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
   using S = AttnShape<T, D, MT, RG, KG, STAGES>;
   static_assert(MINB * (S::SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
 
-  template <bool PAGE16> static cudaError_t start(const AttnParams& p, int dev, cudaStream_t s) {
+  template <bool PAGE16> static cudaError_t start(const AttnParams& p, unsigned grid, int dev, cudaStream_t s) {
     static std::atomic<bool> ready[kMaxDevices];
     auto k = attn_kernel<T, D, MT, RG, KG, STAGES, REGB, PAGE16>;
     if (!ready[dev].load(std::memory_order_acquire)) {
@@ -111,19 +105,23 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
       if (e != cudaSuccess) return e;
       ready[dev].store(true, std::memory_order_release);
     }
-    return launch(k, (unsigned)p.grid, S::THREADS, S::SMEM, s, p);
+    return launch(k, grid, S::THREADS, S::SMEM, s, p);
   }
   static cudaError_t run(AttnParams* p, int dev, AttnPlan* plan, cudaStream_t s, bool plan_only) {
     cudaError_t e = cudaSuccess;
-    plan->grid = MINB * sm_count(dev, &e);
+    const int full = MINB * sm_count(dev, &e);
     if (e != cudaSuccess) return e;
-    plan->R = S::R;
-    plan->ws_bytes = 2ll * plan->grid * S::R * (D + 2) * 4;
+    const long long units = (long long)p->B * p->Hkv * ((p->span * p->group + S::R - 1) / S::R);
+    const long long tiles = ((long long)p->max_blocks * p->block_size + S::TILE - 1) / S::TILE;
+    const bool cut = tiles > (sizeof(T) == 4 ? kUncutTilesF32 : units * 2 >= full && units <= full ? kUncutTilesFull : kUncutTiles);
+    plan->ws_bytes = cut ? 2ll * full * S::R * (D + 2) * 4 : 0;
     if (plan_only) return cudaSuccess;
-    p->grid = plan->grid;
+    p->split = cut && p->ws != nullptr;
+    p->grid = full;
     p->tile = S::TILE;
     p->unit_cost = kUnitCost;
-    e = p->block_size % 16 == 0 ? start<true>(*p, dev, s) : start<false>(*p, dev, s);
+    const unsigned grid = (unsigned)(!p->split && units < full ? units : full);
+    e = p->block_size % 16 == 0 ? start<true>(*p, grid, dev, s) : start<false>(*p, grid, dev, s);
     if (e != cudaSuccess || !p->split) return e;
     const long long rows = (long long)p->T * p->Hq;
     // As many warps per row as one CTA of eight on every SM allows: few rows are cut into many parts each, and a CTA
@@ -137,7 +135,8 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
 
 // Rows that share a kv head's keys: tokens of the span x query heads of the group.  The smallest tile that holds them,
 // at most 64 (32 for heads of 256): more rows than that read the cache once per tile.
-template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int rows, int dev, AttnPlan* plan, cudaStream_t s, bool po) {
+template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int dev, AttnPlan* plan, cudaStream_t s, bool po) {
+  const long long rows = (long long)p->span * p->group;
   if constexpr (sizeof(T) == 4) {
     switch (D) {
       case 32: return AttnVariant<T, 32, 1, 1, 4, 4, 2>::run(p, dev, plan, s, po);
@@ -156,13 +155,9 @@ template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int rows, 
         if (rows <= 32) return AttnVariant<T, 64, 2, 1, 4, 4, 3>::run(p, dev, plan, s, po);
         return AttnVariant<T, 64, 2, 2, 4, 5, 2>::run(p, dev, plan, s, po);
       case 128:
-        if (rows <= 16) return AttnVariant<T, 128, 1, 1, 4, 3, 2, RB>::run(p, dev, plan, s, po);
+        if (rows <= 16) return AttnVariant<T, 128, 1, 1, 4, 3, 2, 3>::run(p, dev, plan, s, po);
         if (rows <= 32) return AttnVariant<T, 128, 2, 1, 4, 3, 2>::run(p, dev, plan, s, po);
-#ifdef R64
-        return AttnVariant<T, 128, 1, 4, 4, 6, 1>::run(p, dev, plan, s, po);
-#else
         return AttnVariant<T, 128, 2, 2, 4, 6, 1>::run(p, dev, plan, s, po);
-#endif
       default:
         if (rows <= 16) return AttnVariant<T, 256, 1, 1, 4, 3, 1>::run(p, dev, plan, s, po);
         return AttnVariant<T, 256, 1, 2, 4, 3, 1>::run(p, dev, plan, s, po);
@@ -170,12 +165,12 @@ template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int rows, 
   }
 }
 
-int run_attn(AttnParams* p, int dtype, int D, int rows, int dev, AttnPlan* plan, cudaStream_t s, bool plan_only, const char* who) {
+int run_attn(AttnParams* p, int dtype, int D, int dev, AttnPlan* plan, cudaStream_t s, bool plan_only, const char* who) {
   cudaError_t e;
   switch (dtype) {
-    case B200MOE_F32: e = dispatch_attn<float>(p, D, rows, dev, plan, s, plan_only); break;
-    case B200MOE_F16: e = dispatch_attn<__half>(p, D, rows, dev, plan, s, plan_only); break;
-    default: e = dispatch_attn<__nv_bfloat16>(p, D, rows, dev, plan, s, plan_only); break;
+    case B200MOE_F32: e = dispatch_attn<float>(p, D, dev, plan, s, plan_only); break;
+    case B200MOE_F16: e = dispatch_attn<__half>(p, D, dev, plan, s, plan_only); break;
+    default: e = dispatch_attn<__nv_bfloat16>(p, D, dev, plan, s, plan_only); break;
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -241,19 +236,20 @@ extern "C" int b200moe_store_kv(const b200moe_store_kv_args* a, void* stream) {
   return B200MOE_OK;
 }
 
-extern "C" int b200moe_paged_attention_workspace(int dtype, int num_heads, int num_kv_heads, int head_dim, int max_query_len, int64_t max_context,
-                                                 int64_t* bytes_out) {
+extern "C" int b200moe_paged_attention_workspace(int dtype, int num_seqs, int num_heads, int num_kv_heads, int head_dim, int max_query_len,
+                                                 int max_blocks_per_seq, int block_size, int64_t* bytes_out) {
   const char* who = "b200moe_paged_attention_workspace";
   if (!bytes_out) return b200moe_fail_global(B200MOE_E_ARG, "%s: null pointer", who);
   if (int rc = check_heads(who, dtype, num_heads, num_kv_heads, head_dim)) return rc;
-  if (max_query_len < 0 || max_context < 0) return b200moe_fail_global(B200MOE_E_ARG, "%s: negative size", who);
+  if (num_seqs < 0 || max_query_len < 0 || max_blocks_per_seq < 0 || block_size <= 0) return b200moe_fail_global(B200MOE_E_ARG, "%s: negative size", who);
   *bytes_out = 0;
-  if (max_context <= kNoSplitSlots) return B200MOE_OK;
   int dev;
   if (int rc = current_device(who, &dev)) return rc;
+  AttnParams p = {};
+  p.B = num_seqs; p.Hkv = num_kv_heads; p.group = num_heads / num_kv_heads; p.span = max_query_len > 0 ? max_query_len : 1;
+  p.max_blocks = max_blocks_per_seq; p.block_size = block_size;
   AttnPlan plan;
-  const long long rows = (long long)max_query_len * (num_heads / num_kv_heads);
-  if (int rc = run_attn(nullptr, dtype, head_dim, (int)(rows < 1024 ? rows : 1024), dev, &plan, nullptr, true, who)) return rc;
+  if (int rc = run_attn(&p, dtype, head_dim, dev, &plan, nullptr, true, who)) return rc;
   *bytes_out = plan.ws_bytes;
   return B200MOE_OK;
 }
@@ -292,16 +288,13 @@ extern "C" int b200moe_paged_attention(const b200moe_paged_attention_args* a, vo
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.B = a->num_seqs; p.T = a->num_tokens; p.Hq = a->num_heads; p.Hkv = a->num_kv_heads; p.group = a->num_heads / a->num_kv_heads;
   p.block_size = a->block_size; p.num_blocks = a->num_blocks; p.max_blocks = a->max_blocks_per_seq;
-  const long long span = a->query_start ? a->max_query_len : 1;
-  const long long rows = span * p.group;
+  p.span = a->query_start && a->max_query_len > 0 ? a->max_query_len : 1;
   AttnPlan plan;
-  const int rows_i = (int)(rows < 1024 ? rows : 1024);
-  p.split = max_context > kNoSplitSlots && a->workspace != nullptr;
-  if (p.split) {
-    if (int rc = run_attn(&p, dt, a->head_dim, rows_i, dev, &plan, nullptr, true, who)) return rc;
+  if (p.ws) {
+    if (int rc = run_attn(&p, dt, a->head_dim, dev, &plan, nullptr, true, who)) return rc;
     if (a->workspace_bytes < plan.ws_bytes)
       return b200moe_fail_global(B200MOE_E_ARG, "%s: workspace of %lld bytes, %lld are needed (b200moe_paged_attention_workspace)", who,
                                  (long long)a->workspace_bytes, (long long)plan.ws_bytes);
   }
-  return run_attn(&p, dt, a->head_dim, rows_i, dev, &plan, (cudaStream_t)stream, false, who);
+  return run_attn(&p, dt, a->head_dim, dev, &plan, (cudaStream_t)stream, false, who);
 }

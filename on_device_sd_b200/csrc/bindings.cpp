@@ -261,7 +261,9 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       s.lse_out = (float*)lse.data_ptr();
     }
     // the workspace belongs to this call: calls on several streams and captured graphs do not share one
-    check(b200moe_paged_attention_workspace(s.dtype, s.num_heads, s.num_kv_heads, s.head_dim, s.max_query_len, width * kc.size(1), &s.workspace_bytes));
+    if (T > 0 && B > 0)
+      check(b200moe_paged_attention_workspace(s.dtype, s.num_seqs, s.num_heads, s.num_kv_heads, s.head_dim, s.max_query_len, s.max_blocks_per_seq,
+                                              s.block_size, &s.workspace_bytes));
     if (s.workspace_bytes) {
       ws = at::empty({s.workspace_bytes}, at::TensorOptions().device(dev).dtype(at::kByte));
       s.workspace = ws.data_ptr();

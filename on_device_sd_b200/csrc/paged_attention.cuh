@@ -42,7 +42,7 @@ struct AttnParams {
   float* ws;                       // parts: [2 * grid][R * D] o, then [2 * grid][R][2] (m, l)
   long long q_tok, q_head, o_tok, o_head, c_block, c_slot, c_head, table_stride;
   float scale_log2;                // scale * log2(e)
-  int B, T, Hq, Hkv, group, block_size, num_blocks, max_blocks;
+  int B, T, Hq, Hkv, group, block_size, num_blocks, max_blocks, span;
   int split;                       // 0: units are not cut
   int tile;                        // keys of a tile
   int unit_cost;                   // what beginning a unit costs, in tiles
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   if (p.status)
     for (int b = blockIdx.x * THREADS + tid; b < p.B; b += gridDim.x * THREADS) attn_report(p, b);
   const long long W = attn_work_before(p, p.B, R);
-  const int g = (int)(W < p.grid ? W : p.grid);
+  const int g = (int)(W < gridDim.x ? W : gridDim.x);
   const int cta = blockIdx.x;
   if (cta >= g) return;
   long long lo = attn_lo(W, g, cta);

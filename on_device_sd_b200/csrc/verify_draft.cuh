@@ -59,29 +59,46 @@ template <typename T, int E, bool VEC> __device__ __forceinline__ void load_prob
   }
 }
 
-// r_i of the draw: what is left of p after the draft's share, never negative; `skip` is a token that has none.  Which
-// elements count is decided in fp32, where the comparison is exact and a NaN counts as nothing; the rest is in 64 bits.
-template <typename T, int E, bool VEC>
+// r_i of the draw: what is left of p after the draft's share q (LESS), never negative; `skip` is a token that has none.
+// Which elements count is decided in fp32, where the comparison is exact and a NaN counts as nothing; the rest is in
+// 64 bits.
+template <typename T, int E, bool VEC, bool LESS>
 __device__ __forceinline__ void load_rest(const T* p, const T* q, int skip, int i, int end, double (&r)[E]) {
   float f[E];
   load_probs<T, E, VEC>(p, i, end, f);
-  if (q) {
+  if constexpr (LESS) {
     float s[E];
     load_probs<T, E, VEC>(q, i, end, s);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-      const bool left = f[k] > s[k] && f[k] > 0.0f;
+      const bool left = f[k] > s[k];
       r[k] = (double)(left ? f[k] : 0.0f) - (double)(left ? s[k] : 0.0f);
     }
   } else {
 #pragma unroll
     for (int k = 0; k < E; ++k) r[k] = (double)fmaxf(f[k], 0.0f);
-  }
-  if ((unsigned)(skip - i) < (unsigned)E) {
+    if ((unsigned)(skip - i) < (unsigned)E) {
 #pragma unroll
-    for (int k = 0; k < E; ++k)
-      if (i + k == skip) r[k] = 0.0;
+      for (int k = 0; k < E; ++k)
+        if (i + k == skip) r[k] = 0.0;
+    }
   }
+}
+
+// The sum of r over [lo, hi), by a whole warp.
+template <typename T, bool VEC, bool LESS> __device__ __forceinline__ double rest_sum(const T* p, const T* q, int skip, int lo, int hi) {
+  constexpr int E = 16 / (int)sizeof(T);
+  double sum = 0.0;
+#pragma unroll 4
+  for (int i = lo + (threadIdx.x & 31) * E; i < hi; i += 32 * E) {
+    double r[E];
+    load_rest<T, E, VEC, LESS>(p, q, skip, i, hi, r);
+    double part = 0.0;
+#pragma unroll
+    for (int k = 0; k < E; ++k) part += r[k];
+    sum += part;
+  }
+  return warp_sum(sum);
 }
 
 // The first of up to 2 x 32 sums (two per lane, in index order) with which the running sum passes `goal`, and the sum
@@ -175,15 +192,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_draft_kernel(const V
   const int lo = (int)min((long long)piece * per, (long long)p.V), hi = min(lo + per, p.V);
 
   for (int round = 0; round < 2; ++round) {
-    double sum = 0.0;
-#pragma unroll 4
-    for (int i = lo + lane * E; i < hi; i += UNIT) {
-      double r[E];
-      load_rest<T, E, VEC>(row, less, skip, i, hi, r);
-#pragma unroll
-      for (int k = 0; k < E; ++k) sum += r[k];
-    }
-    sum = warp_sum(sum);
+    double sum = less ? rest_sum<T, VEC, true>(row, less, skip, lo, hi) : rest_sum<T, VEC, false>(row, less, skip, lo, hi);
     if (round == 0) cluster.barrier_wait();
     if (lane < C) *cluster.map_shared_rank(&s_sum[round][piece], lane) = sum;
     cluster.sync();
@@ -204,14 +213,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_draft_kernel(const V
     const int plo = (int)min((long long)f.at * per, (long long)p.V), phi = min(plo + per, p.V);
     const int share = ((phi - plo + kVerifyWarps - 1) / kVerifyWarps + E - 1) / E * E;
     const int slo = min(plo + warp * share, phi), shi = min(slo + share, phi);
-    sum = 0.0;
-    for (int i = slo + lane * E; i < shi; i += UNIT) {
-      double r[E];
-      load_rest<T, E, VEC>(row, less, skip, i, shi, r);
-#pragma unroll
-      for (int k = 0; k < E; ++k) sum += r[k];
-    }
-    sum = warp_sum(sum);
+    sum = less ? rest_sum<T, VEC, true>(row, less, skip, slo, shi) : rest_sum<T, VEC, false>(row, less, skip, slo, shi);
     if (lane == 0) s_part[warp] = sum;
     __syncthreads();
     const Found w = find_sum(lane < kVerifyWarps / 2 ? s_part[2 * lane] : 0.0, lane < kVerifyWarps / 2 ? s_part[2 * lane + 1] : 0.0, f.before, 0.0, false,
@@ -225,7 +227,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_draft_kernel(const V
       double r[E], s = 0.0;
 #pragma unroll
       for (int k = 0; k < E; ++k) r[k] = 0.0;
-      if (i < shi) load_rest<T, E, VEC>(row, less, skip, i, shi, r);
+      if (i < shi) {
+        if (less) load_rest<T, E, VEC, true>(row, less, skip, i, shi, r);
+        else load_rest<T, E, VEC, false>(row, less, skip, i, shi, r);
+      }
 #pragma unroll
       for (int k = 0; k < E; ++k) s += r[k];
       const double inc = warp_scan_incl(s);

@@ -98,10 +98,13 @@ def test_null_arguments_and_empty_calls():
     assert lib.b200moe_paged_attention(ctypes.byref(attn_args(num_tokens=0, num_seqs=0)), None) == _lib.OK
     assert lib.b200moe_verify_draft(ctypes.byref(verify_args(num_seqs=0)), None) == _lib.OK
     n = ctypes.c_int64(-1)
-    assert lib.b200moe_paged_attention_workspace(_lib.BF16, 32, 4, 128, 1, 100, ctypes.byref(n)) == _lib.OK and n.value == 0
-    assert lib.b200moe_paged_attention_workspace(_lib.BF16, 32, 4, 128, 1, 100, None) == _lib.E_ARG
-    assert lib.b200moe_paged_attention_workspace(_lib.BF16, 32, 5, 128, 1, 100, ctypes.byref(n)) == _lib.E_ARG
-    assert lib.b200moe_paged_attention_workspace(_lib.BF16, 32, 4, 128, -1, 100, ctypes.byref(n)) == _lib.E_ARG
+    ws = lib.b200moe_paged_attention_workspace
+    assert ws(_lib.BF16, 1, 32, 4, 128, 1, 4, 16, None) == _lib.E_ARG
+    assert ws(_lib.BF16, 1, 32, 5, 128, 1, 4, 16, ctypes.byref(n)) == _lib.E_ARG
+    assert ws(_lib.BF16, 1, 32, 4, 128, -1, 4, 16, ctypes.byref(n)) == _lib.E_ARG
+    assert ws(_lib.BF16, -1, 32, 4, 128, 1, 4, 16, ctypes.byref(n)) == _lib.E_ARG
+    assert ws(_lib.BF16, 1, 32, 4, 128, 1, 4, 0, ctypes.byref(n)) == _lib.E_ARG
+    assert ws(_lib.BF16, 1, 32, 4, 100, 1, 4, 16, ctypes.byref(n)) == _lib.E_UNSUPPORTED
 
 
 def test_argument_structs_have_the_headers_layout(tmp_path):
