@@ -133,8 +133,10 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
   }
 };
 
-// Rows that share a kv head's keys: tokens of the span x query heads of the group.  The smallest tile that holds them,
-// at most 64 (32 for heads of 256): more rows than that read the cache once per tile.
+// Rows that share a kv head's keys: tokens of the span x query heads of the group, in tiles of 16 or 32.  More than 32
+// read the cache once per tile, the further times from L2: a tile of 64 rows would leave one CTA of 8 warps on an SM and
+// was slower (64 spans of 1..5 tokens, 8 heads a group, over ~8000: 343 us against 229; 64 rows everywhere: equal).
+// Heads of 256 need two warps' registers for 32 rows (32 spans of 4 over 10000: 77 us, with tiles of 16 rows 105).
 template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int dev, AttnPlan* plan, cudaStream_t s, bool po) {
   const long long rows = (long long)p->span * p->group;
   if constexpr (sizeof(T) == 4) {
@@ -148,16 +150,13 @@ template <typename T> cudaError_t dispatch_attn(AttnParams* p, int D, int dev, A
     switch (D) {
       case 32:
         if (rows <= 16) return AttnVariant<T, 32, 1, 1, 4, 6, 4>::run(p, dev, plan, s, po);
-        if (rows <= 32) return AttnVariant<T, 32, 2, 1, 4, 6, 3>::run(p, dev, plan, s, po);
-        return AttnVariant<T, 32, 2, 2, 4, 6, 2>::run(p, dev, plan, s, po);
+        return AttnVariant<T, 32, 2, 1, 4, 6, 3>::run(p, dev, plan, s, po);
       case 64:
         if (rows <= 16) return AttnVariant<T, 64, 1, 1, 4, 4, 3>::run(p, dev, plan, s, po);
-        if (rows <= 32) return AttnVariant<T, 64, 2, 1, 4, 4, 3>::run(p, dev, plan, s, po);
-        return AttnVariant<T, 64, 2, 2, 4, 5, 2>::run(p, dev, plan, s, po);
+        return AttnVariant<T, 64, 2, 1, 4, 4, 3>::run(p, dev, plan, s, po);
       case 128:
         if (rows <= 16) return AttnVariant<T, 128, 1, 1, 4, 3, 2, 3>::run(p, dev, plan, s, po);
-        if (rows <= 32) return AttnVariant<T, 128, 2, 1, 4, 3, 2>::run(p, dev, plan, s, po);
-        return AttnVariant<T, 128, 2, 2, 4, 6, 1>::run(p, dev, plan, s, po);
+        return AttnVariant<T, 128, 2, 1, 4, 3, 2>::run(p, dev, plan, s, po);
       default:
         if (rows <= 16) return AttnVariant<T, 256, 1, 1, 4, 3, 1>::run(p, dev, plan, s, po);
         return AttnVariant<T, 256, 1, 2, 4, 3, 1>::run(p, dev, plan, s, po);

@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         if (t1 <= t0) continue;    // only the part that stands for the beginning
       }
       u->first = sq.first; u->ctx = sq.ctx; u->n = sq.n;
-      u->head = unit % p.Hkv;
-      u->row0 = unit / p.Hkv * R;
+      u->head = unit / sq.row_tiles;   // row tiles of one head follow each other: the second finds the cache in L2
+      u->row0 = unit % sq.row_tiles * R;
       u->rows = min(R, sq.n * p.group - u->row0);
       u->tile0 = t0; u->ntile = t1 - t0;
       // a part that begins inside a unit is this CTA's first, one that ends inside a unit its last
@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int 
       const int g = (int)(W < p.grid ? W : p.grid);
       const int head = h / p.group, r_all = (token - sq.first) * p.group + h % p.group;
       r = r_all % R;
-      const long long u0 = attn_work_before(p, b, R) + (long long)(r_all / R * p.Hkv + head) * attn_weight(p, sq) + p.unit_cost;
+      const long long u0 = attn_work_before(p, b, R) + (long long)(head * sq.row_tiles + r_all / R) * attn_weight(p, sq) + p.unit_cost;
       c0 = attn_owner(W, g, u0);
       c1 = attn_owner(W, g, u0 + sq.tiles - 1);
       cut = c0 != c1;                                                 // else one CTA has written the output
