@@ -68,7 +68,7 @@ def _build_step(force: bool, verbose: bool) -> None:
     cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
     cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(tdir / "include"), "-isystem", str(cuda / "include"),
-           str(src), "-o", str(STEP), "-L", str(tdir / "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda",
+           str(src), "-o", str(STEP), "-L", str(tdir / "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda",
            "-L", str(PKG), "-lb200moe", "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:

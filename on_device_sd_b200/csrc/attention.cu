@@ -286,7 +286,7 @@ extern "C" int b200moe_paged_attention(const b200moe_paged_attention_args* a, vo
   p.c_block = a->cache_block_stride; p.c_slot = a->cache_slot_stride; p.c_head = a->cache_head_stride; p.table_stride = a->block_table_stride;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.B = a->num_seqs; p.T = a->num_tokens; p.Hq = a->num_heads; p.Hkv = a->num_kv_heads; p.group = a->num_heads / a->num_kv_heads;
-  p.block_size = a->block_size; p.num_blocks = a->num_blocks; p.max_blocks = a->max_blocks_per_seq;
+  p.block_size = a->block_size; p.num_blocks = a->num_blocks; p.max_blocks = has_cache ? a->max_blocks_per_seq : 0;
   p.span = a->query_start && a->max_query_len > 0 ? a->max_query_len : 1;
   AttnPlan plan;
   if (p.ws) {

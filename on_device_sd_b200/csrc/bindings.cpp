@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -117,8 +118,10 @@ void cache_pair(const at::Tensor& k, const at::Tensor& v, c10::Device dev, at::S
     refuse(PyExc_ValueError, "the caches must be [blocks, block_size, kv_heads, " + std::to_string(head_dim) + "] with contiguous heads, got " + shape_text(k.sizes()));
   if (k.size(1) == 0) refuse(PyExc_ValueError, "the caches need a block size of at least one slot");
 }
+// torch.empty without the way through the dispatcher
+at::Tensor empty(c10::Device dev, at::ScalarType dtype, at::IntArrayRef shape) { return at::detail::empty_cuda(shape, dtype, dev, std::nullopt); }
 at::Tensor output(PyObject* o, c10::Device dev, at::ScalarType dtype, at::IntArrayRef shape) {
-  if (o == Py_None) return at::empty(shape, at::TensorOptions().device(dev).dtype(dtype));
+  if (o == Py_None) return empty(dev, dtype, shape);
   const at::Tensor& t = tensor(o, "out");
   need(t, "out", dev, dtype, 3);
   if (t.sizes() != shape || (t.stride(2) != 1 && shape[2] > 1))
@@ -257,7 +260,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor out = output(a[8], dev, dt, query.sizes()), lse, ws;
     s.out = out.data_ptr(); s.o_token_stride = out.stride(0); s.o_head_stride = out.stride(1);
     if (with_lse) {
-      lse = at::empty({T, hq}, at::TensorOptions().device(dev).dtype(at::kFloat));
+      lse = empty(dev, at::kFloat, {T, hq});
       s.lse_out = (float*)lse.data_ptr();
     }
     // the workspace belongs to this call: calls on several streams and captured graphs do not share one
@@ -265,7 +268,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       check(b200moe_paged_attention_workspace(s.dtype, s.num_seqs, s.num_heads, s.num_kv_heads, s.head_dim, s.max_query_len, s.max_blocks_per_seq,
                                               s.block_size, &s.workspace_bytes));
     if (s.workspace_bytes) {
-      ws = at::empty({s.workspace_bytes}, at::TensorOptions().device(dev).dtype(at::kByte));
+      ws = empty(dev, at::kByte, {s.workspace_bytes});
       s.workspace = ws.data_ptr();
     }
     check(b200moe_paged_attention(&s, c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
@@ -315,8 +318,8 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.num_seqs = int32(B, "the number of sequences"); s.vocab_size = int32(vocab, "the vocabulary"); s.max_draft_len = int32(longest, "max_draft_len");
     s.num_draft_tokens = int32(drafts, "the number of drafts"); s.num_target_rows = int32(target.size(0), "the number of target rows");
     const c10::cuda::CUDAGuard guard(dev);
-    at::Tensor out = at::empty({B, longest + 1}, at::TensorOptions().device(dev).dtype(at::kLong));
-    at::Tensor count = at::empty({B}, at::TensorOptions().device(dev).dtype(at::kInt));
+    at::Tensor out = empty(dev, at::kLong, {B, longest + 1});
+    at::Tensor count = empty(dev, at::kInt, {B});
     s.tokens_out = (int64_t*)out.data_ptr(); s.accepted_out = (int32_t*)count.data_ptr();
     check(b200moe_verify_draft(&s, c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
     PyObject *o = THPVariable_Wrap(std::move(out)), *c = THPVariable_Wrap(std::move(count));

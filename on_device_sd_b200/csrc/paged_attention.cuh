@@ -566,65 +566,65 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         }
       }
     } else {
-      // fp32: lane = key for the scores (32/KEYS groups of rows), lane = D/32 columns for the second product
-      constexpr int RPL = 16 * KEYS / 32;                             // score rows of a lane
+      // fp32: for the scores a lane is one key and every other row, for the second product D/32 columns and all rows.  What
+      // bounds it are the loads from shared memory (five of 16 bytes for 16 products), so rows go in groups of 4, 8 or 16
+      // and are not padded to 16 as on the tensor cores.
       constexpr int C = D / 32;                                       // output columns of a lane
       float* s_p = reinterpret_cast<float*>(smem + S::P_OFF) + kg * (KEYS + 1) * 16;
       float* s_f = s_p + KEYS * 16;
-      const int key_l = lane % KEYS, rbase = (lane / KEYS) * RPL;
-      float o[16][C], m[RPL], l[RPL];
+      const int key_l = lane % 16, half = lane / 16;                  // score rows half, half + 2, ...
+      const int my_limit = limit(key_l);                              // of row lane % 16
+      float o[16][C], m[8], l[8];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
 #pragma unroll
         for (int i = 0; i < C; ++i) o[r][i] = 0.0f;
 #pragma unroll
-      for (int r = 0; r < RPL; ++r) { m[r] = -INFINITY; l[r] = 0.0f; }
+      for (int i = 0; i < 8; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
       const unsigned char* s_q = smem + S::Q_OFF + qbuf * S::QB;
-      for (int t = 0; t < u.ntile; ++t) {
-        cp_async_wait<STAGES - 2>();
-        __syncwarp();
-        issue(u, t + STAGES - 1, slot_after(at, STAGES - 1));
-        const unsigned char* ks_base = smem + (ring - sbase) + at * S::SLOT;
-        at = slot_after(at, 1);
+      // One stage for the first 2 * NP rows
+      auto stage = [&](auto pairs, const unsigned char* ks_base, int key0) {
+        constexpr int NP = decltype(pairs)::value;
         const unsigned char* vs_base = ks_base + S::HALF_STAGE;
-        const int key0 = (u.tile0 + t) * S::TILE + kg * KEYS;
-        if (key0 >= u.ctx) continue;
-        float s[RPL];
+        float s[NP];
 #pragma unroll
-        for (int r = 0; r < RPL; ++r) s[r] = 0.0f;
+        for (int i = 0; i < NP; ++i) s[i] = 0.0f;
 #pragma unroll 4
         for (int ch = 0; ch < CPR; ++ch) {
           const float4 kv = *reinterpret_cast<const float4*>(ks_base + row_chunk<ROWB>(key_l, ch));
 #pragma unroll
-          for (int r = 0; r < RPL; ++r) {
-            const float4 qv = *reinterpret_cast<const float4*>(s_q + row_chunk<ROWB>(rbase + r, ch));
-            s[r] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[r]))));
+          for (int i = 0; i < NP; ++i) {
+            const float4 qv = *reinterpret_cast<const float4*>(s_q + row_chunk<ROWB>(2 * i + half, ch));
+            s[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[i]))));
           }
         }
         const bool masked = key0 + KEYS > lim0;
 #pragma unroll
-        for (int r = 0; r < RPL; ++r) {
-          float x = s[r];
-          if (masked && key0 + key_l >= limit(rbase + r)) x = -INFINITY;
-          float top = x * p.scale_log2;
+        for (int i = 0; i < NP; ++i) {
+          if (masked) {
+            const int lim = __shfl_sync(0xffffffffu, my_limit, 2 * i + half);
+            if (key0 + key_l >= lim) s[i] = -INFINITY;
+          }
+          float top = s[i] * p.scale_log2;
 #pragma unroll
-          for (int w = KEYS / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-          const float mn = fmaxf(m[r], top);
+          for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          const float mn = fmaxf(m[i], top);
           const float ref = mn == -INFINITY ? 0.0f : mn;
-          const float f = ex2(m[r] - ref);
-          m[r] = mn;
-          x = ex2(fmaf(x, p.scale_log2, -ref));
-          l[r] = l[r] * f + x;
-          s_p[key_l * 16 + rbase + r] = x;
-          if (key_l == 0) s_f[rbase + r] = f;
+          const float f = ex2(m[i] - ref);
+          m[i] = mn;
+          const float x = ex2(fmaf(s[i], p.scale_log2, -ref));
+          l[i] = l[i] * f + x;
+          s_p[key_l * 16 + 2 * i + half] = x;
+          if (key_l == 0) s_f[2 * i + half] = f;
         }
         __syncwarp();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
+        for (int r = 0; r < 2 * NP; ++r) {
           const float f = s_f[r];
 #pragma unroll
           for (int i = 0; i < C; ++i) o[r][i] *= f;
         }
+#pragma unroll 2
         for (int j = 0; j < KEYS; ++j) {
           float v[C];
 #pragma unroll
@@ -633,26 +633,48 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
             const int col = lane * C + i;
             v[i] = *reinterpret_cast<const float*>(vs_base + row_chunk<ROWB>(j, col / 4) + (col % 4) * 4);
           }
+          float w[2 * NP];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            // rows that do not see the key are left alone (0 * inf is not 0)
-            if (!masked || key0 + j < limit(r)) {
-              const float w = s_p[j * 16 + r];
+          for (int r = 0; r < 2 * NP; r += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(s_p + j * 16 + r);
+            w[r] = x.x; w[r + 1] = x.y; w[r + 2] = x.z; w[r + 3] = x.w;
+          }
+          // rows that do not see the key are left alone (0 * inf is not 0)
+          const unsigned seen = masked ? __ballot_sync(0xffffffffu, key0 + j < my_limit) : 0xffffffffu;
+          if (seen == 0xffffffffu) {
 #pragma unroll
-              for (int i = 0; i < C; ++i) o[r][i] = fmaf(w, v[i], o[r][i]);
-            }
+            for (int r = 0; r < 2 * NP; ++r)
+#pragma unroll
+              for (int i = 0; i < C; ++i) o[r][i] = fmaf(w[r], v[i], o[r][i]);
+          } else if (seen) {
+#pragma unroll
+            for (int r = 0; r < 2 * NP; ++r)
+#pragma unroll
+              for (int i = 0; i < C; ++i) o[r][i] = (seen >> r) & 1 ? fmaf(w[r], v[i], o[r][i]) : o[r][i];
           }
         }
         __syncwarp();
+      };
+      for (int t = 0; t < u.ntile; ++t) {
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();
+        issue(u, t + STAGES - 1, slot_after(at, STAGES - 1));
+        const unsigned char* base = smem + (ring - sbase) + at * S::SLOT;
+        at = slot_after(at, 1);
+        const int key0 = (u.tile0 + t) * S::TILE + kg * KEYS;
+        if (key0 >= u.ctx) continue;
+        if (rows <= 4) stage(std::integral_constant<int, 2>{}, base, key0);
+        else if (rows <= 8) stage(std::integral_constant<int, 4>{}, base, key0);
+        else stage(std::integral_constant<int, 8>{}, base, key0);
       }
       more = next_unit(&nu);
       if (more) begin(nu, at, qbuf ^ 1);
 #pragma unroll
-      for (int r = 0; r < RPL; ++r) {
-        float sum = l[r];
+      for (int i = 0; i < 8; ++i) {
+        float sum = l[i];
 #pragma unroll
-        for (int w = KEYS / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        if (key_l == 0) s_ml[kg * R + rbase + r] = make_float2(m[r], sum);
+        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (key_l == 0) s_ml[kg * R + 2 * i + half] = make_float2(m[i], sum);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r)
