@@ -320,7 +320,7 @@ int b200moe_store_kv(const b200moe_store_kv_args* args, void* stream);
  * context_lens[b] - n + i + 1 keys.
  *   out[t,h] = sum_j softmax_j(scale * q[t,h] . k[j]) v[j];  lse_out[t,h] = log sum_j exp(scale * q . k[j])
  * A row that sees no key gives zeros and -inf.  Keys that a row does not see do not reach it whatever they hold.
- * Rows behind query_start[num_seqs] are left as they were.  Page indices outside [0, num_blocks) are not followed
+ * Rows behind query_start[num_seqs] are left as they were.  out may be query itself.  Page indices outside [0, num_blocks) are not followed
  * (B200MOE_DEV_BAD_PAGE; that sequence's output is not to be used); lengths that do not fit the tensors are cut, and
  * spans that do not are skipped (B200MOE_DEV_BAD_LENGTH).
  * max_query_len: the longest span; longer ones are computed correctly, but read the cache more often.

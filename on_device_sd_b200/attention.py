@@ -57,5 +57,5 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     value gives right results.  scale defaults to D ** -0.5.
 
     Returns out [T, heads, D] (with return_lse also the fp32 log-sum-exp [T, heads]).  A row that sees no key gives zeros
-    and -inf; rows behind query_start[B] are not written (nor initialised unless `out` was given)."""
+    and -inf; rows behind query_start[B] are not written (nor initialised unless `out` was given).  `out` may be `query`."""
     return load_step().paged_attention(query, k_cache, v_cache, block_tables, context_lens, query_start, max_query_len, scale, out, return_lse, status)

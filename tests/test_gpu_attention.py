@@ -483,3 +483,29 @@ def test_store_then_attention_follow_each_other():
     c.q, c.kc, c.vc, c.tables = qr, kc2, vc2, tables
     c.check(got)
     c.check(c.run())
+
+
+def test_output_in_the_queries_place():
+    """out may be the query tensor itself, cut along the cache or not."""
+    for contexts in ([40, 3], [5000, 900]):
+        c = Case(BF16, 32, 4, 128, 16, [5, 9], contexts, seed=40)
+        want = c.run().clone()
+        q = c.q
+        assert c.run(out=q) is q and torch.equal(q, want)
+
+
+def test_graph_pool_shared_by_two_graphs():
+    """Two graphs captured into one memory pool and replayed one after the other, as an engine keeps one per batch size."""
+    cases = [Case(BF16, 32, 4, 128, 256, [1] * n, [3000] * n, seed=41 + n) for n in (1, 4)]
+    want = [c.run(query_start=None).clone() for c in cases]
+    pool = torch.cuda.graph_pool_handle()
+    graphs, outs = [], []
+    for c in cases:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, pool=pool):
+            outs.append(c.run(query_start=None))
+        graphs.append(gr)
+    for i in (0, 1, 1, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want[i])
