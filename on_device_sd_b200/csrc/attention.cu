@@ -118,18 +118,18 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
     if (plan_only) return cudaSuccess;
     p->split = cut && p->ws != nullptr;
     p->grid = full;
-    p->tile = S::TILE;
+    p->tile_shift = S::TILE == 64 ? 6 : 5;
+    static_assert(S::TILE == 64 || S::TILE == 32, "tile");
     p->unit_cost = kUnitCost;
     const unsigned grid = (unsigned)(!p->split && units < full ? units : full);
     e = p->block_size % 16 == 0 ? start<true>(*p, grid, dev, s) : start<false>(*p, grid, dev, s);
     if (e != cudaSuccess || !p->split) return e;
     const long long rows = (long long)p->T * p->Hq;
-    // As many warps per row as one CTA of eight on every SM allows: few rows are cut into many parts each, and a CTA
-    // that fits beside the attention kernel's has begun when that one ends.
-    if (rows <= 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R);
-    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), 256, 0, s, *p, S::R);
-    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), 256, 0, s, *p, S::R);
-    return launch(attn_join_kernel<T, D, 1>, (unsigned)((rows + 7) / 8), 256, 0, s, *p, S::R);
+    // Few rows are cut into many parts each: up to eight warps per row, in up to two CTAs of eight on every SM.
+    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R_SHIFT);
+    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), 256, 0, s, *p, S::R_SHIFT);
+    if (rows <= 8 * 148) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), 256, 0, s, *p, S::R_SHIFT);
+    return launch(attn_join_kernel<T, D, 1>, (unsigned)((rows + 7) / 8), 256, 0, s, *p, S::R_SHIFT);
   }
 };
 

@@ -44,7 +44,7 @@ struct AttnParams {
   float scale_log2;                // scale * log2(e)
   int B, T, Hq, Hkv, group, block_size, num_blocks, max_blocks, span;
   int split;                       // 0: units are not cut
-  int tile;                        // keys of a tile
+  int tile_shift;                  // a tile holds 1 << tile_shift keys
   int unit_cost;                   // what beginning a unit costs, in tiles
   int grid;                        // CTAs of the attention kernel
 };
@@ -56,7 +56,7 @@ struct AttnSeq {
   int first, n, ctx;               // first query row, new tokens, keys
   int row_tiles, tiles;
 };
-__device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b, int R) {
+__device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b, int r_shift) {   // a row tile holds 1 << r_shift rows
   AttnSeq s;
   s.first = b; s.n = 1;
   s.ctx = p.context[b];
@@ -69,8 +69,8 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b, int R) {
   const long long cap = (long long)p.max_blocks * p.block_size;
   if (s.ctx < 0) s.ctx = 0;
   if (s.ctx > cap) s.ctx = (int)cap;
-  s.row_tiles = (s.n * p.group + R - 1) / R;
-  s.tiles = max((s.ctx + p.tile - 1) / p.tile, 1);   // an empty sequence still has rows to write
+  s.row_tiles = (s.n * p.group + (1 << r_shift) - 1) >> r_shift;
+  s.tiles = max((s.ctx + (1 << p.tile_shift) - 1) >> p.tile_shift, 1);   // an empty sequence still has rows to write
   return s;
 }
 __device__ __forceinline__ void attn_report(const AttnParams& p, int b) {
@@ -91,18 +91,18 @@ __device__ __forceinline__ long long warp_sum_ll(long long v) {
   return v;
 }
 // Work of the sequences [0, b_end), by a whole warp.
-__device__ __forceinline__ long long attn_work_before(const AttnParams& p, int b_end, int R) {
+__device__ __forceinline__ long long attn_work_before(const AttnParams& p, int b_end, int r_shift) {
   long long w = 0;
-  for (int b = threadIdx.x & 31; b < b_end; b += 32) w += attn_work(p, attn_seq(p, b, R));
+  for (int b = threadIdx.x & 31; b < b_end; b += 32) w += attn_work(p, attn_seq(p, b, r_shift));
   return warp_sum_ll(w);
 }
 // The sequence that holds work item x, and the work before it; by a whole warp.
-__device__ __forceinline__ int attn_find(const AttnParams& p, long long x, int R, long long* before) {
+__device__ __forceinline__ int attn_find(const AttnParams& p, long long x, int r_shift, long long* before) {
   const int lane = threadIdx.x & 31;
   long long base = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
-    const long long w = b < p.B ? attn_work(p, attn_seq(p, b, R)) : 0;
+    const long long w = b < p.B ? attn_work(p, attn_seq(p, b, r_shift)) : 0;
     long long inc = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -120,9 +120,13 @@ __device__ __forceinline__ int attn_find(const AttnParams& p, long long x, int R
   *before = base;
   return p.B;
 }
+// Division of numbers that are seldom past 32 bits, where it takes a fifth of the time.
+__device__ __forceinline__ long long div_ll(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
 // CTA c of g takes the items [attn_lo(c), attn_lo(c+1)); item x belongs to CTA attn_owner(x).  g <= W.
-__device__ __forceinline__ long long attn_lo(long long W, int g, int c) { return W * c / g; }
-__device__ __forceinline__ int attn_owner(long long W, int g, long long x) { return (int)(((x + 1) * g - 1) / W); }
+__device__ __forceinline__ long long attn_lo(long long W, int g, int c) { return div_ll(W * c, g); }
+__device__ __forceinline__ int attn_owner(long long W, int g, long long x) { return (int)div_ll((x + 1) * g - 1, W); }
 
 // ---------------------------------------------------------------------------------------------
 // Primitives
@@ -182,6 +186,8 @@ template <int ROWB> __device__ __forceinline__ uint32_t row_chunk(int row, int c
 // MT: 16-row tiles of a warp, RG: row groups (warps that share a ring), KG: key groups.
 template <typename T, int D, int MT, int RG, int KG, int STAGES_> struct AttnShape {
   static constexpr int R = 16 * MT * RG;
+  static constexpr int R_SHIFT = R == 16 ? 4 : 5;
+  static_assert(R == 1 << R_SHIFT, "rows");
   static constexpr int STAGES = STAGES_;
   static constexpr int KEYS = 16;                  // keys of a stage
   static constexpr int TILE = KEYS * KG;
@@ -207,7 +213,7 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES_> struct AttnSha
 template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, bool PAGE16>
 __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnParams p) {
   using S = AttnShape<T, D, MT, RG, KG, STAGES>;
-  constexpr int R = S::R, ROWB = S::ROWB, CPR = S::CPR, KEYS = S::KEYS, THREADS = S::THREADS;
+  constexpr int R = S::R, RS = S::R_SHIFT, ROWB = S::ROWB, CPR = S::CPR, KEYS = S::KEYS, THREADS = S::THREADS;
   constexpr bool kMma = sizeof(T) == 2;
   static_assert(kMma || (MT == 1 && RG == 1), "shape");
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -221,14 +227,14 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   pdl_trigger();                   // after the wait: the join may then read this call's lengths before its own wait
   if (p.status)
     for (int b = blockIdx.x * THREADS + tid; b < p.B; b += gridDim.x * THREADS) attn_report(p, b);
-  const long long W = attn_work_before(p, p.B, R);
+  const long long W = attn_work_before(p, p.B, RS);
   const int g = (int)(W < gridDim.x ? W : gridDim.x);
   const int cta = blockIdx.x;
   if (cta >= g) return;
   long long lo = attn_lo(W, g, cta);
   const long long hi = attn_lo(W, g, cta + 1);
   long long seq_base;
-  int b_next = attn_find(p, lo, R, &seq_base);
+  int b_next = attn_find(p, lo, RS, &seq_base);
   const T* kc = reinterpret_cast<const T*>(p.k);
   const T* vc = reinterpret_cast<const T*>(p.v);
 
@@ -241,11 +247,11 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   };
   auto next_unit = [&](Unit* u) -> bool {
     while (lo < hi && b_next < p.B) {
-      const AttnSeq sq = attn_seq(p, b_next, R);
+      const AttnSeq sq = attn_seq(p, b_next, RS);
       const long long seq_work = attn_work(p, sq);
       if (lo >= seq_base + seq_work) { seq_base += seq_work; ++b_next; continue; }
       const int weight = attn_weight(p, sq);
-      const int unit = (int)((lo - seq_base) / weight), skip = (int)((lo - seq_base) % weight);
+      const int unit = (int)div_ll(lo - seq_base, weight), skip = (int)(lo - seq_base - (long long)unit * weight);
       const int take = (int)min(hi - lo, (long long)(weight - skip));
       lo += take;
       int t0 = 0, t1 = sq.tiles;
@@ -729,15 +735,16 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
 // its own wait, so the lengths are complete.  No warp leaves before the wait - the next kernel takes the end of this
 // grid for the end of both.
 template <typename T, int D, int WPR>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int R) {
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int r_shift) {
   constexpr int RPC = 8 / WPR;
   constexpr int C = D / 32;
+  const int R = 1 << r_shift;
   __shared__ float s_acc[WPR > 1 ? 8 : 1][D];
   __shared__ float2 s_ml[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
-  const long long row = (long long)blockIdx.x * RPC + warp / WPR;     // (token, head)
-  const int token = (int)(row / p.Hq), h = (int)(row % p.Hq);
+  const unsigned row = blockIdx.x * RPC + warp / WPR;                 // (token, head), below 2^31
+  const int token = (int)(row / (unsigned)p.Hq), h = (int)(row - (unsigned)token * p.Hq);
   bool cut = token < p.T;
   int b = token;
   if (cut && p.qstart) {
@@ -751,14 +758,14 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int 
   cut = cut && b < p.B;
   int c0 = 0, c1 = 0, r = 0;
   if (cut) {
-    const AttnSeq sq = attn_seq(p, b, R);
+    const AttnSeq sq = attn_seq(p, b, r_shift);
     cut = token >= sq.first && token < sq.first + sq.n;
     if (cut) {
-      const long long W = attn_work_before(p, p.B, R);
+      const long long W = attn_work_before(p, p.B, r_shift);
       const int g = (int)(W < p.grid ? W : p.grid);
       const int head = h / p.group, r_all = (token - sq.first) * p.group + h % p.group;
-      r = r_all % R;
-      const long long u0 = attn_work_before(p, b, R) + (long long)(head * sq.row_tiles + r_all / R) * attn_weight(p, sq) + p.unit_cost;
+      r = r_all & (R - 1);
+      const long long u0 = attn_work_before(p, b, r_shift) + (long long)(head * sq.row_tiles + (r_all >> r_shift)) * attn_weight(p, sq) + p.unit_cost;
       c0 = attn_owner(W, g, u0);
       c1 = attn_owner(W, g, u0 + sq.tiles - 1);
       cut = c0 != c1;                                                 // else one CTA has written the output
