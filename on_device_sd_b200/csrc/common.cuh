@@ -36,6 +36,17 @@ template <typename T> __device__ __forceinline__ float rn(float v) {
 }
 template <> __device__ __forceinline__ float rn<float>(float v) { return v; }
 
+// Two values rounded and packed by one instruction, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // ---------------------------------------------------------------------------------------------
 // A "chunk" is 8 consecutive elements: one 16-byte load for 16-bit types, two for fp32.
 // ---------------------------------------------------------------------------------------------

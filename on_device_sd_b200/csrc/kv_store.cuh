@@ -9,8 +9,8 @@
 // What bounds it: one launch for the few tokens of a decoding step, HBM for a prompt.  D/16 lanes hold one head, each
 // lane 8 elements of either half, so a rotation pairs registers of one lane, loads are 16 bytes and the norm's sum is
 // a few shuffles.  A lane group takes kHeads heads of one token after the other and keeps the token's angles in
-// registers: the fp32 table row is twice a 16-bit head.  8191 tokens of 32 + 2 x 8 heads of 128, fp16, take 37.6 us
-// (5.5 TB/s) with four heads, 39.1 us with two, 47.7 us with eight.
+// registers: the fp32 table row is twice a 16-bit head.  8191 tokens of 32 + 2 x 8 heads of 128, fp16, take 35.7 us
+// (5.8 TB/s) with four heads; two were 4 % and eight 27 % slower.
 #pragma once
 #include "common.cuh"
 
@@ -41,14 +41,11 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* dst, const 
     reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
     reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
   } else {
-    T v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::from_float(f[i]);
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
   }
 }
 
-constexpr int kStoreThreads = 256;
+constexpr int kStoreThreads = 64;     // small CTAs: 8191 tokens 35.7 us, with 128 threads 36.5, with 256 37.8
 
 // Heads 0..Hq-1 are queries, then Hkv keys, then Hkv values.  Lane group = (token, kHeads consecutive heads).
 template <typename T, int D, int kHeads>

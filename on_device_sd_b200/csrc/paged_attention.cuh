@@ -162,15 +162,6 @@ template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], cons
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 template <typename T> __device__ __forceinline__ bool any_nonfinite2(uint32_t x) {   // either of two packed 16-bit values
   const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   return (x & e) == e || ((x >> 16) & e) == e;
@@ -385,7 +376,6 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
       const int mts = min(MT, ((rows + 15) / 16 - rg + RG - 1) / RG);
       float o[MT][D / 8][4];
       float m[MT][2], l[MT][2];
-      int lim[MT][2];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -393,7 +383,6 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           m[mt][hh] = -INFINITY; l[mt][hh] = 0.0f;
-          lim[mt][hh] = limit((mt * RG + rg) * 16 + hh * 8 + (lane >> 2));
         }
       }
       // Fragment addresses: a step of 16 columns is two chunks, and an exclusive or with it keeps the permutation.
@@ -434,13 +423,17 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         }
 
         const bool masked = key0 + KEYS > lim0;
+        // keys that this lane's row hh of row tile mt sees (recomputed in the few stages that need it: registers are scarce)
+        auto row_limit = [&](int mt, int hh) { return limit((mt * RG + rg) * 16 + hh * 8 + (lane >> 2)); };
         if (masked) {
 #pragma unroll
           for (int mt = 0; mt < M; ++mt)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int key = key0 + (i >> 2) * 8 + 2 * (lane & 3) + (i & 1);
-              if (key >= lim[mt][(i >> 1) & 1]) s[mt][i >> 2][i & 3] = -INFINITY;
+            for (int hh = 0; hh < 2; ++hh) {
+              const int lim = row_limit(mt, hh);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (key0 + (i >> 1) * 8 + 2 * (lane & 3) + (i & 1) >= lim) s[mt][i >> 1][2 * hh + (i & 1)] = -INFINITY;
             }
         }
         // m is the reference that p is taken against: a maximum of the row that is renewed only when the row has
@@ -513,6 +506,9 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
             }
           }
         } else {
+          int lim[M][2];
+#pragma unroll
+          for (int mt = 0; mt < M; ++mt) { lim[mt][0] = row_limit(mt, 0); lim[mt][1] = row_limit(mt, 1); }
 #pragma unroll 1
           for (int j = 0; j < KEYS; ++j) {
             // this lane holds keys 2*(lane%4), +1 (registers 0, 1 of A; 0, 2 of B) and those + 8 (2, 3; 1, 3)
@@ -814,8 +810,17 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int 
   if (!cut) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   T* dst = reinterpret_cast<T*>(p.out) + token * p.o_tok + h * p.o_head + lane * C;
+  if constexpr (sizeof(T) == 2 && C >= 2) {
+    uint32_t v[C / 2];
 #pragma unroll
-  for (int i = 0; i < C; ++i) dst[i] = Elem<T>::from_float(acc[i] * inv);
+    for (int i = 0; i < C / 2; ++i) v[i] = pack2<T>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    if constexpr (C == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+    else if constexpr (C == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) dst[i] = Elem<T>::from_float(acc[i] * inv);
+  }
   if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
 }
 
