@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -111,7 +112,9 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
     cudaError_t e = cudaSuccess;
     const int full = MINB * sm_count(dev, &e);
     if (e != cudaSuccess) return e;
-    const long long units = (long long)p->B * p->Hkv * ((p->span * p->group + S::R - 1) / S::R);
+    // as far as comparisons need them
+    const long long row_tiles = std::min(((long long)p->span * p->group + S::R - 1) / S::R, 1ll << 20);
+    const long long units = (long long)std::min(p->B, 1 << 24) * p->Hkv * row_tiles;
     const long long tiles = ((long long)p->max_blocks * p->block_size + S::TILE - 1) / S::TILE;
     const bool cut = tiles > (sizeof(T) == 4 ? kUncutTilesF32 : units * 2 >= full && units <= full ? kUncutTilesFull : kUncutTiles);
     plan->ws_bytes = cut ? 2ll * full * S::R * (D + 2) * 4 : 0;
@@ -272,7 +275,7 @@ extern "C" int b200moe_paged_attention(const b200moe_paged_attention_args* a, vo
                              a->cache_head_stride};
   for (int64_t s : strides)
     if (odd_stride(s, dt)) return b200moe_fail_global(B200MOE_E_ARG, "%s: strides must be multiples of 16 bytes", who);
-  if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return b200moe_fail_global(B200MOE_E_ARG, "%s: scale must be positive and finite", who);
+  if (!(a->scale > 0.0f) || a->scale > 1.0e30f) return b200moe_fail_global(B200MOE_E_ARG, "%s: scale must be positive and at most 1e30", who);
   const int64_t max_context = (int64_t)a->max_blocks_per_seq * a->block_size;
   if (max_context > (1ll << 30)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: block tables span more than 2^30 slots", who);
   // the join's grid and the row numbers are 32-bit

@@ -68,6 +68,15 @@ int int32(int64_t v, const char* name) {
   return (int)v;
 }
 
+// The stride of a dimension; of one with a single entry it says nothing and may be anything.
+int64_t step(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+// A tensor that is written has a place of its own for every entry (expanded dimensions do not).
+void own_places(const at::Tensor& t, const char* name) {
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) == 0) refuse(PyExc_ValueError, std::string(name) + " is written and must not be an expanded tensor, got strides " + shape_text(t.strides()));
+}
+
 // --- checks -----------------------------------------------------------------------------------
 int dtype_tag(const at::Tensor& t, const char* name) {
   int tag = -1;
@@ -113,7 +122,8 @@ void heads_contiguous(const at::Tensor& t, const char* name) {
 void cache_pair(const at::Tensor& k, const at::Tensor& v, c10::Device dev, at::ScalarType dtype, int64_t head_dim) {
   need(k, "k_cache", dev, dtype, 4);
   need(v, "v_cache", dev, dtype, 4);
-  if (k.sizes() != v.sizes() || k.strides() != v.strides()) refuse(PyExc_ValueError, "k_cache and v_cache must have the same shape and strides");
+  if (k.sizes() != v.sizes() || step(k, 0) != step(v, 0) || step(k, 1) != step(v, 1) || step(k, 2) != step(v, 2) || k.stride(3) != v.stride(3))
+    refuse(PyExc_ValueError, "k_cache and v_cache must have the same shape and strides");
   if (k.size(3) != head_dim || k.stride(3) != 1)
     refuse(PyExc_ValueError, "the caches must be [blocks, block_size, kv_heads, " + std::to_string(head_dim) + "] with contiguous heads, got " + shape_text(k.sizes()));
   if (k.size(1) == 0) refuse(PyExc_ValueError, "the caches need a block size of at least one slot");
@@ -126,6 +136,7 @@ at::Tensor output(PyObject* o, c10::Device dev, at::ScalarType dtype, at::IntArr
   need(t, "out", dev, dtype, 3);
   if (t.sizes() != shape || (t.stride(2) != 1 && shape[2] > 1))
     refuse(PyExc_ValueError, "out must be " + shape_text(shape) + " with contiguous heads, got " + shape_text(t.sizes()));
+  own_places(t, "out");
   return t;
 }
 
@@ -180,12 +191,14 @@ PyObject* store_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t T = key.size(0), hk = key.size(1), D = key.size(2);
     cache_pair(kc, vc, dev, dt, D);
     if (kc.size(2) != hk) refuse(PyExc_ValueError, "the caches hold " + std::to_string(kc.size(2)) + " key-value heads, key and value " + std::to_string(hk));
+    own_places(kc, "k_cache");
+    own_places(vc, "v_cache");
     heads_contiguous(key, "key");
     heads_contiguous(value, "value");
     s.slots = index(tensor(a[7], "slot_mapping"), "slot_mapping", dev, T, &s.slots_are_int64);
     s.key = key.data_ptr(); s.value = value.data_ptr(); s.k_cache = kc.data_ptr(); s.v_cache = vc.data_ptr();
-    s.k_token_stride = key.stride(0); s.k_head_stride = key.stride(1); s.v_token_stride = value.stride(0); s.v_head_stride = value.stride(1);
-    s.cache_block_stride = kc.stride(0); s.cache_slot_stride = kc.stride(1); s.cache_head_stride = kc.stride(2);
+    s.k_token_stride = step(key, 0); s.k_head_stride = step(key, 1); s.v_token_stride = step(value, 0); s.v_head_stride = step(value, 1);
+    s.cache_block_stride = step(kc, 0); s.cache_slot_stride = step(kc, 1); s.cache_head_stride = step(kc, 2);
     s.num_tokens = int32(T, "the number of tokens"); s.num_kv_heads = int32(hk, "kv_heads"); s.head_dim = int32(D, "head_dim");
     s.num_blocks = int32(kc.size(0), "the number of blocks"); s.block_size = int32(kc.size(1), "the block size");
     at::Tensor out;
@@ -196,7 +209,7 @@ PyObject* store_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
       heads_contiguous(*query, "query");
       out = output(a[11], dev, dt, query->sizes());
       s.query = query->data_ptr(); s.query_out = out.data_ptr(); s.num_heads = int32(query->size(1), "heads");
-      s.q_token_stride = query->stride(0); s.q_head_stride = query->stride(1); s.o_token_stride = out.stride(0); s.o_head_stride = out.stride(1);
+      s.q_token_stride = step(*query, 0); s.q_head_stride = step(*query, 1); s.o_token_stride = step(out, 0); s.o_head_stride = step(out, 1);
     }
     if (table) {
       need(*table, "cos_sin", dev, at::kFloat, 2);
@@ -249,8 +262,8 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (with_lse < 0) return nullptr;
     s.status = status_ptr(a[10], dev);
     s.query = query.data_ptr(); s.k_cache = kc.data_ptr(); s.v_cache = vc.data_ptr(); s.block_tables = (const int32_t*)tables.data_ptr();
-    s.q_token_stride = query.stride(0); s.q_head_stride = query.stride(1);
-    s.cache_block_stride = kc.stride(0); s.cache_slot_stride = kc.stride(1); s.cache_head_stride = kc.stride(2); s.block_table_stride = tables.stride(0);
+    s.q_token_stride = step(query, 0); s.q_head_stride = step(query, 1);
+    s.cache_block_stride = step(kc, 0); s.cache_slot_stride = step(kc, 1); s.cache_head_stride = step(kc, 2); s.block_table_stride = step(tables, 0);
     s.num_tokens = int32(T, "the number of tokens"); s.num_seqs = int32(B, "the number of sequences");
     s.num_heads = int32(hq, "heads"); s.num_kv_heads = int32(kc.size(2), "kv_heads"); s.head_dim = int32(D, "head_dim");
     s.num_blocks = int32(kc.size(0), "the number of blocks"); s.block_size = int32(kc.size(1), "the block size");
@@ -258,7 +271,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.scale = (float)scale;
     const c10::cuda::CUDAGuard guard(dev);
     at::Tensor out = output(a[8], dev, dt, query.sizes()), lse, ws;
-    s.out = out.data_ptr(); s.o_token_stride = out.stride(0); s.o_head_stride = out.stride(1);
+    s.out = out.data_ptr(); s.o_token_stride = step(out, 0); s.o_head_stride = step(out, 1);
     if (with_lse) {
       lse = empty(dev, at::kFloat, {T, hq});
       s.lse_out = (float*)lse.data_ptr();

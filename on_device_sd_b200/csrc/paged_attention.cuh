@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   int page_next = 0;
   auto lookup = [&](const Unit& u, int t) {                           // page of this lane's key of tile t (one stage ahead)
     const int key = (u.tile0 + t) * S::TILE + kg * KEYS + (PAGE16 ? 0 : lane % KEYS);
-    page_next = (t < u.ntile && key < u.ctx) ? __ldg(u.table + key / p.block_size) : -1;
+    page_next = (t < u.ntile && key < u.ctx) ? u.table[key / p.block_size] : -1;
   };
   auto issue = [&](const Unit& u, int t, int slot_at) {
     if (t < u.ntile) {

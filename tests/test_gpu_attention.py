@@ -382,6 +382,12 @@ def test_refuses_what_does_not_fit():
         paged_attention(shifted, *ok[1:])
     with pytest.raises(_lib.B200MoEError, match="head_dim"):
         paged_attention(c.q[..., :96], c.kc[..., :96], c.vc[..., :96], c.tables, c.lens)
+    with pytest.raises(ValueError, match="expanded"):
+        paged_attention(*ok, out=torch.zeros(1, 8, 128, dtype=BF16, device="cuda").expand(2, 8, 128))
+    kv = torch.zeros(2, 2, 128, dtype=BF16, device="cuda")
+    flat = torch.zeros(1, 16, 2, 128, dtype=BF16, device="cuda").expand(3, 16, 2, 128)
+    with pytest.raises(ValueError, match="expanded"):
+        store_kvcache(kv, kv, flat, flat, torch.tensor([0, 40], device="cuda"))
     odd = torch.zeros(2, 7, 128, dtype=BF16, device="cuda")
     with pytest.raises(_lib.B200MoEError, match="multiple"):
         paged_attention(odd, *ok[1:])
@@ -509,3 +515,20 @@ def test_graph_pool_shared_by_two_graphs():
         graphs[i].replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[i], want[i])
+
+
+def test_strides_of_single_entries_do_not_matter():
+    """One token, one kv head, one block: the stride of such a dimension may be any number."""
+    c = Case(BF16, 4, 1, 64, 16, [1], [16], seed=50, poison=False)
+    kc, vc = c.kc[c.tables[0, 0].long()][None].contiguous(), c.vc[c.tables[0, 0].long()][None].contiguous()
+    q = c.q[:1].contiguous()
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    want = paged_attention(q, kc, vc, table, c.lens)
+    q2 = q.as_strided((1, 4, 64), (3, 64, 1))
+    k2, v2 = kc.as_strided((1, 16, 1, 64), (5, 64, 7, 1)), vc.as_strided((1, 16, 1, 64), (1, 64, 9, 1))
+    assert torch.equal(paged_attention(q2, k2, v2, table.as_strided((1, 1), (77, 55)), c.lens), want)
+    before = kc.clone()
+    store_kvcache(q[:, :1].as_strided((1, 1, 64), (1, 3, 1)), q[:, 1:2], k2, v2, torch.tensor([5], device="cuda"))
+    assert torch.equal(kc[0, 5, 0], q[0, 0]) and torch.equal(vc[0, 5, 0], q[0, 1])
+    kc[0, 5] = before[0, 5]
+    assert torch.equal(kc, before)
