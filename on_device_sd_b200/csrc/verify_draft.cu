@@ -18,7 +18,7 @@ template <typename T> cudaError_t launch_verify(const VerifyParams& p, cudaStrea
   cudaLaunchConfig_t cfg = {};
   // eight CTAs per sequence until four on every SM (what the registers allow) are taken, fewer for larger batches
   unsigned cluster = kVerifyMaxCluster;
-  while (cluster > 1 && (long long)p.B * cluster > 4 * 148) cluster /= 2;
+  while (cluster > 1 && (long long)p.B * cluster > kVerifyCtasPerSm * 148) cluster /= 2;
   cfg.gridDim = dim3((unsigned)p.B * cluster);
   cfg.blockDim = dim3(kVerifyThreads);
   cfg.stream = s;
