@@ -125,6 +125,11 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
     static_assert(S::TILE == 64 || S::TILE == 32, "tile");
     p->unit_cost = kUnitCost;
     const unsigned grid = (unsigned)(!p->split && units < full ? units : full);
+    // division by the page size as a multiplication, exact for keys below 2^31: page_mul = floor(2^(31+s) / d) + 1, 2^s >= d
+    int sh = 0;
+    while ((1ll << sh) < p->block_size) ++sh;
+    p->page_shift = 31 + sh;
+    p->page_mul = (unsigned)((1ull << (31 + sh)) / (unsigned)p->block_size + 1);
     e = p->block_size % 16 == 0 ? start<true>(*p, grid, dev, s) : start<false>(*p, grid, dev, s);
     if (e != cudaSuccess || !p->split) return e;
     const long long rows = (long long)p->T * p->Hq;

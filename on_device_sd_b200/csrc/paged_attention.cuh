@@ -51,6 +51,8 @@ struct AttnParams {
   float scale_log2;                // scale * log2(e)
   int B, T, Hq, Hkv, group, block_size, num_blocks, max_blocks, span;
   int split;                       // 0: units are not cut
+  unsigned page_mul;               // key / block_size = key * page_mul >> page_shift, for keys below 2^31
+  int page_shift;
   int tile_shift;                  // a tile holds 1 << tile_shift keys
   int unit_cost;                   // what beginning a unit costs, in tiles
   int grid;                        // CTAs of the attention kernel
@@ -276,9 +278,10 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   constexpr int COPIES = (KEYS * CPR + STEP - 1) / STEP;
   const int pt = rg * 32 + lane;
   int page_next = 0;                                                  // page of the next stage to fetch, looked up one stage ahead
+  auto block_of = [&](int key) -> int { return (int)(((unsigned long long)(unsigned)key * p.page_mul) >> p.page_shift); };
   auto page_of = [&](const Unit& u, int t) -> int {                   // of this lane's key of tile t
     const int key = (u.tile0 + t) * S::TILE + kg * KEYS + (PAGE16 ? 0 : lane % KEYS);
-    return (t < u.ntile && key < u.ctx) ? u.table[key / p.block_size] : -1;
+    return (t < u.ntile && key < u.ctx) ? u.table[block_of(key)] : -1;
   };
   auto issue = [&](const Unit& u, int t, int slot_at, int page) {
     if (t < u.ntile) {
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
       const bool in = key < u.ctx;
       const bool ok = in && page >= 0 && page < p.num_blocks;
       if (in && !ok && p.status) atomicOr(p.status, kDevBadPage);
-      const long long off = ok ? page * p.c_block + (long long)(key % p.block_size) * p.c_slot : 0;
+      const long long off = ok ? page * p.c_block + (long long)(key - block_of(key) * p.block_size) * p.c_slot : 0;
       if constexpr (PAGE16) {
         // a lane's rows are STEP/CPR apart at one chunk (or, in rows longer than a step, its chunks STEP apart)
         constexpr int DROW = CPR <= STEP ? STEP / CPR : 0;
