@@ -70,14 +70,15 @@ template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, 
 // b200moe_paged_attention
 // ---------------------------------------------------------------------------------------------
 // Whether a call's units are cut along the cache over the whole grid, from what the host knows: B sequences of at most
-// max_blocks * block_size slots.  Uncut, a unit belongs to one CTA, which takes about 1 us for a tile (4 us in fp32) when it
-// has the time to itself; cut, a second kernel joins the parts, about 2 us.  16-bit types, 4 kv heads, us uncut / cut:
-// one sequence of 33 slots 5.5 / 7.2, of 200 8.6 / 7.2 (so 4 tiles, half of them used on average, go uncut); 16 of up to
-// 200 7.7 / 9.8.  Units that just fill the GPU once gain longer: 64 sequences of up to 500 slots 14.6 / 16.5, of 1000
-// 24.1 / 21.6; with 8 kv heads, more units than fit at once, 25.5 / 23.2 at 500.
+// max_blocks * block_size slots.  Uncut, a unit belongs to one CTA, which takes about 0.9 us for a tile when it has the
+// time to itself; cut, a second kernel joins the parts.  16-bit types, heads of 128, 4 kv heads, us uncut / cut: one
+// sequence of 33 slots 5.5 / 6.1, of 120 6.4 / 6.8, of 250 8.0 / 6.7 (tables are as wide as the pages, lengths lie
+// anywhere below: on average 4 tiles break even); 16 sequences of 250 8.2 / 9.0.  Units that just fill the GPU once gain
+// longer: 64 sequences of 500 13.3 / 16.4; of 1000, cut, 29.1; with 8 kv heads, more units than fit at once, 29.9 / 29.7 at
+// 500.  fp32: 60 slots 5.9 / 6.6, 120 slots 8.5 / 7.0.
 constexpr int kUncutTiles = 4, kUncutTilesFull = 8, kUncutTilesF32 = 1;
 // What beginning a unit costs a CTA, in tiles of 64 keys, for the equal division of the work.  (32 spans over 100..2500
-// tokens: 55.2 us at 0, 48.0 at 1, 44.2 at 2, 42.8 at 3; equal lengths do not care.)
+// tokens: 55 us at 0, 48 at 1, 44 at 2, 43 at 3; equal lengths do not care.)
 constexpr int kUnitCost = 3;
 
 struct AttnPlan {

@@ -1,7 +1,7 @@
 // Python entry of the step operators: on_device_sd_b200/_step.so, called by attention.py and speculative.py.
 //
 // A draft step's kernels take a few microseconds, and checking a dozen tensors, filling the argument struct and
-// allocating from Python takes 8-10 (measured with ctypes; 3 here).  So these functions take the tensors themselves:
+// allocating from Python takes 8-10 (measured with ctypes; about 2 here).  So these functions take the tensors themselves:
 // they check devices, types, shapes and strides, allocate the outputs and the workspace from torch's allocator, and call
 // the C ABI (include/b200moe.h) on the current stream of the tensors' device.  No arithmetic happens here.
 #include <Python.h>

@@ -26,10 +26,12 @@
 // (the operand type of the tensor cores; the sum l uses the same unrounded p), outputs are rounded once.
 //
 // Measured on B200, device time back to back, heads of 128: 32 sequences of 21000 tokens, 8 kv heads of 4 queries 405 us
-// (6.8 TB/s, the copy rate), with spans of 8 tokens 430 us; one sequence of 131071, 4 kv heads 50 us (5.4 TB/s); 16 of
-// 300..6000 26.5 us (4.5 TB/s); 64 spans of 1..5 tokens, 8 queries a kv head, over 800..16384 tokens 232 us.  What is
+// (6.8 TB/s, the copy rate), with spans of 8 tokens 430 us; one sequence of 131071, 4 kv heads 50.8 us (5.3 TB/s); 16 of
+// 300..6000 25.4 us (4.7 TB/s); 64 spans of 1..5 tokens, 8 queries a kv head, over 800..16384 tokens 228 us.  What is
 // left there is fixed cost: about 5 us from the launch to the first products (lengths, page table and cache are three
-// dependent loads), about 3 us for the join.
+// dependent loads), about 3 us for the join.  A stage of 16 keys is some 1600 cycles of dependent instructions for its
+// warp whatever is in flight, which eight warps an SM hide for 16 rows and just about for 32.  Slower were: bulk copies of a
+// row per lane (by 10 to 30 %), rows padded in shared memory instead of permuted (3 to 9 %), a deeper ring (nothing).
 #pragma once
 #include <type_traits>
 

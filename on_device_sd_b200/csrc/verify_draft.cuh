@@ -11,9 +11,9 @@
 // shared memory over the cluster, and the CTA whose piece holds the draw reads it again (from L2), all its warps side by
 // side, to find the token.  One launch, no workspace, no atomics in global memory.
 //
-// Measured on B200, device time back to back: one sequence of 4 drafts over 32000 tokens 5.8 us, of which about 3.5 are
-// that chain; 48 sequences over 151936 13.0 us (58 MB where every draft is refused: 4.5 TB/s); 64 greedy ones over
-// 128256, bf16, 9.8 us, which the conversions to 64 bits bound (16 per clock and SM).
+// Measured on B200, device time back to back: one sequence of 4 drafts over 32000 tokens 5.2 us, of which about 3 are
+// that chain; 48 sequences over 151936 15.7 us with new inputs every call (12.3 us from L2); 64 greedy ones over
+// 128256, bf16, 9.5 us, which the conversions to 64 bits bound (16 per clock and SM).
 #pragma once
 #include <cooperative_groups.h>
 
