@@ -75,7 +75,7 @@ template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, 
 // sequence of 33 slots 5.5 / 6.1, of 120 6.4 / 6.8, of 250 8.0 / 6.7 (tables are as wide as the pages, lengths lie
 // anywhere below: on average 4 tiles break even); 16 sequences of 250 8.2 / 9.0.  Units that just fill the GPU once gain
 // longer: 64 sequences of 500 13.3 / 16.4; of 1000, cut, 29.1; with 8 kv heads, more units than fit at once, 29.9 / 29.7 at
-// 500.  fp32: 60 slots 5.9 / 6.6, 120 slots 8.5 / 7.0.
+// 500.  fp32: one sequence of 60 slots 5.9 / 6.6; past a tile its products alone take longer than the join.
 constexpr int kUncutTiles = 4, kUncutTilesFull = 8, kUncutTilesF32 = 1;
 // What beginning a unit costs a CTA, in tiles of 64 keys, for the equal division of the work.  (32 spans over 100..2500
 // tokens: 55 us at 0, 48 at 1, 44 at 2, 43 at 3; equal lengths do not care.)
