@@ -322,7 +322,8 @@ int b200moe_store_kv(const b200moe_store_kv_args* args, void* stream);
  * A row that sees no key gives zeros and -inf.  Keys that a row does not see do not reach it whatever they hold.
  * Rows behind query_start[num_seqs] are left as they were.  out may be query itself.  Page indices outside [0, num_blocks) are not followed
  * (B200MOE_DEV_BAD_PAGE; that sequence's output is not to be used); lengths that do not fit the tensors are cut, and
- * spans that do not are skipped (B200MOE_DEV_BAD_LENGTH).
+ * spans that do not are skipped (B200MOE_DEV_BAD_LENGTH); the other sequences are served all the same, and a row that two
+ * of them claim gets the output of either.
  * max_query_len: the longest span; longer ones are computed correctly, but read the cache more often.
  * workspace: as many bytes as b200moe_paged_attention_workspace gives for the same numbers on the same device (0 for
  * short contexts; max_query_len is 1 without query_start); it need not be cleared and must not be shared by calls that

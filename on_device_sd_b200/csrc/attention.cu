@@ -117,8 +117,8 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
     const long long row_tiles = std::min(((long long)p->span * p->group + S::R - 1) / S::R, 1ll << 20);
     const long long units = (long long)std::min(p->B, 1 << 24) * p->Hkv * row_tiles;
     const long long tiles = ((long long)p->max_blocks * p->block_size + S::TILE - 1) / S::TILE;
-    const bool cut = tiles > (sizeof(T) == 4 ? kUncutTilesF32 : units * 2 >= full && units <= full ? kUncutTilesFull : kUncutTiles);
-    plan->ws_bytes = cut ? 2ll * full * S::R * (D + 2) * 4 : 0;
+    const bool cut = full <= kJoinMaxGrid && tiles > (sizeof(T) == 4 ? kUncutTilesF32 : units * 2 >= full && units <= full ? kUncutTilesFull : kUncutTiles);
+    plan->ws_bytes = cut ? attn_ws_floats(full, S::R, D) * 4 : 0;
     if (plan_only) return cudaSuccess;
     p->split = cut && p->ws != nullptr;
     p->grid = full;
@@ -133,12 +133,12 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
     p->page_mul = (unsigned)((1ull << (31 + sh)) / (unsigned)p->block_size + 1);
     e = p->block_size % 16 == 0 ? start<true>(*p, grid, dev, s) : start<false>(*p, grid, dev, s);
     if (e != cudaSuccess || !p->split) return e;
-    const long long rows = (long long)p->T * p->Hq;
+    const long long rows = std::min((long long)p->T * p->Hq, (long long)(full - 1) * S::R);   // no more are cut: one unit a CTA
     // Few rows are cut into many parts each: up to eight warps per row, in up to two CTAs of eight on every SM.
-    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R_SHIFT);
-    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), 256, 0, s, *p, S::R_SHIFT);
-    if (rows <= 8 * 148) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), 256, 0, s, *p, S::R_SHIFT);
-    return launch(attn_join_kernel<T, D, 1>, (unsigned)((rows + 7) / 8), 256, 0, s, *p, S::R_SHIFT);
+    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, kJoinThreads, 0, s, *p, S::R_SHIFT);
+    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), kJoinThreads, 0, s, *p, S::R_SHIFT);
+    if (rows <= 8 * 148) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), kJoinThreads, 0, s, *p, S::R_SHIFT);
+    return launch(attn_join_kernel<T, D, 1>, (unsigned)((rows + 7) / 8), kJoinThreads, 0, s, *p, S::R_SHIFT);
   }
 };
 

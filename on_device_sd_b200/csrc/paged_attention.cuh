@@ -48,7 +48,7 @@ struct AttnParams {
   const int* context;              // [B]
   const int* qstart;               // [B+1] or null: one token per sequence
   int* status;                     // may be null
-  float* ws;                       // parts: [2 * grid][R * D] o, then [2 * grid][R][2] (m, l)
+  float* ws;                       // parts: [2 * grid][R * D] o, [2 * grid][R][2] (m, l), then [grid] AttnCut and [grid] their spans
   long long q_tok, q_head, o_tok, o_head, c_block, c_slot, c_head, table_stride;
   float scale_log2;                // scale * log2(e)
   int B, T, Hq, Hkv, group, block_size, num_blocks, max_blocks, span;
@@ -93,6 +93,18 @@ __device__ __forceinline__ void attn_report(const AttnParams& p, int b) {
   }
   if (bad) atomicOr(p.status, kDevBadLength);
 }
+// What the join has to know of a unit that goes on behind the CTA that began it: where its rows lie, and in one word
+// how many there are and which CTA took the last of its tiles (rows | CTA << 8).  Every CTA leaves these: none begins
+// more than one such unit, and one that begins none says so (0 rows), so the workspace need not be cleared.
+struct __align__(16) AttnCut {
+  int first, row0, head, unused;   // the sequence's first query row, the unit's first row in it, its kv head
+};
+constexpr int kJoinThreads = 256;
+constexpr int kJoinMaxGrid = 4 * kJoinThreads;                         // a thread of the join takes four of the words
+__host__ __device__ constexpr long long attn_ml_at(int grid, int R, int D) { return 2ll * grid * R * D; }     // in floats
+__host__ __device__ constexpr long long attn_cut_at(int grid, int R, int D) { return 2ll * grid * R * (D + 2); }
+__host__ __device__ constexpr long long attn_span_at(int grid, int R, int D) { return attn_cut_at(grid, R, D) + 4ll * grid; }
+__host__ __device__ constexpr long long attn_ws_floats(int grid, int R, int D) { return attn_span_at(grid, R, D) + (grid + 3) / 4 * 4; }
 // A unit weighs its tiles and the cost of beginning it (the weight's first items stand for that).
 __device__ __forceinline__ int attn_weight(const AttnParams& p, const AttnSeq& s) { return p.split ? s.tiles + p.unit_cost : 1; }
 __device__ __forceinline__ long long attn_work(const AttnParams& p, const AttnSeq& s) { return (long long)s.row_tiles * p.Hkv * attn_weight(p, s); }
@@ -226,13 +238,16 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   float2* s_ml = reinterpret_cast<float2*>(smem + S::ML_OFF);
 
   pdl_wait();
-  pdl_trigger();                   // after the wait: the join may then read this call's lengths before its own wait
+  pdl_trigger();
   if (p.status)
     for (int b = blockIdx.x * THREADS + tid; b < p.B; b += gridDim.x * THREADS) attn_report(p, b);
   const long long W = attn_work_before(p, p.B, RS);
   const int g = (int)(W < gridDim.x ? W : gridDim.x);
   const int cta = blockIdx.x;
-  if (cta >= g) return;
+  if (cta >= g) {
+    if (p.split && tid == 0) reinterpret_cast<int*>(p.ws + attn_span_at(p.grid, R, D))[cta] = 0;
+    return;
+  }
   long long lo = attn_lo(W, g, cta);
   const long long hi = attn_lo(W, g, cta + 1);
   long long seq_base;
@@ -374,6 +389,19 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   bool more = next_unit(&u);
   int at = 0, qbuf = 0;                                               // ring slot of the stage in hand, buffer of the queries
   if (more) begin(u, at, qbuf);
+  if (p.split && warp == 0) {      // while the first loads are under way: the unit that this CTA begins and does not end
+    long long base;
+    const AttnSeq sq = attn_seq(p, attn_find(p, hi - 1, RS, &base), RS);
+    const int weight = attn_weight(p, sq), unit = (int)div_ll(hi - 1 - base, weight);
+    const long long tiles_at = base + (long long)unit * weight + p.unit_cost;     // work item of its first tile
+    const bool cut = hi > tiles_at && hi < tiles_at + sq.tiles && attn_lo(W, g, cta) <= tiles_at;
+    if (lane == 0) {
+      const int row_first = unit % sq.row_tiles * R;
+      const int last = cut ? attn_owner(W, g, tiles_at + sq.tiles - 1) : 0;
+      if (cut) reinterpret_cast<AttnCut*>(p.ws + attn_cut_at(p.grid, R, D))[cta] = AttnCut{sq.first, row_first, unit / sq.row_tiles, 0};
+      reinterpret_cast<int*>(p.ws + attn_span_at(p.grid, R, D))[cta] = cut ? last << 8 | min(R, sq.n * p.group - row_first) : 0;
+    }
+  }
   while (more) {
 #pragma unroll
     for (int t = S::AHEAD; t < STAGES - 1; ++t) {
@@ -736,7 +764,7 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
         if (p.lse && c == 0) p.lse[(long long)token * p.Hq + h] = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
       } else {
         *reinterpret_cast<float4*>(p.ws + ((long long)u.part * R + r) * D + c * 4) = acc;
-        if (c == 0) reinterpret_cast<float2*>(p.ws + 2ll * p.grid * R * D)[(long long)u.part * R + r] = make_float2(top, l);
+        if (c == 0) reinterpret_cast<float2*>(p.ws + attn_ml_at(p.grid, R, D))[(long long)u.part * R + r] = make_float2(top, l);
       }
     }
     qbuf ^= 1;
@@ -745,64 +773,46 @@ __global__ void __launch_bounds__(32 * KG * RG, MINB) attn_kernel(const AttnPara
   }
 }
 
-// Joins the parts of the units that attn_kernel cut.  WPR warps (1, 2, 4 or 8) of the CTA's 8 share an output row.  What
-// depends on the lengths alone is found out before the wait for attn_kernel: that kernel lets this one start only after
-// its own wait, so the lengths are complete.  No warp leaves before the wait - the next kernel takes the end of this
-// grid for the end of both.
+// One row of the join, by WPR warps: the CTA that began its unit (-1: no row here), the row in the unit, and the CTA that
+// ended it.
 template <typename T, int D, int WPR>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int r_shift) {
-  constexpr int RPC = 8 / WPR;
+__device__ __forceinline__ void join_row(const AttnParams& p, int R, int c0, int r, int c1, float (*s_acc)[D], float2* s_ml) {
   constexpr int C = D / 32;
-  const int R = 1 << r_shift;
-  __shared__ float s_acc[WPR > 1 ? 8 : 1][D];
-  __shared__ float2 s_ml[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_trigger();
-  const unsigned row = blockIdx.x * RPC + warp / WPR;                 // (token, head), below 2^31
-  const int token = (int)(row / (unsigned)p.Hq), h = (int)(row - (unsigned)token * p.Hq);
-  bool cut = token < p.T;
-  int b = token;
-  if (cut && p.qstart) {
-    int a = 0, e = p.B;                                               // last b with qstart[b] <= token
-    while (e - a > 1) {
-      const int mid = (a + e) >> 1;
-      if (p.qstart[mid] <= token) a = mid; else e = mid;
-    }
-    b = a;
-  }
-  cut = cut && b < p.B;
-  int c0 = 0, c1 = 0, r = 0;
-  if (cut) {
-    const AttnSeq sq = attn_seq(p, b, r_shift);
-    cut = token >= sq.first && token < sq.first + sq.n;
-    if (cut) {
-      const long long W = attn_work_before(p, p.B, r_shift);
-      const int g = (int)(W < p.grid ? W : p.grid);
-      const int head = h / p.group, r_all = (token - sq.first) * p.group + h % p.group;
-      r = r_all & (R - 1);
-      const long long u0 = attn_work_before(p, b, r_shift) + (long long)(head * sq.row_tiles + (r_all >> r_shift)) * attn_weight(p, sq) + p.unit_cost;
-      c0 = attn_owner(W, g, u0);
-      c1 = attn_owner(W, g, u0 + sq.tiles - 1);
-      cut = c0 != c1;                                                 // else one CTA has written the output
-    }
-  }
-  pdl_wait();
+  const AttnCut u = c0 >= 0 ? reinterpret_cast<const AttnCut*>(p.ws + attn_cut_at(p.grid, R, D))[c0] : AttnCut{0, 0, 0, 0};
   float top = -INFINITY, l = 0.0f;
   float acc[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) acc[i] = 0.0f;
-  if (cut) {
-    const float2* parts_ml = reinterpret_cast<const float2*>(p.ws + 2ll * p.grid * R * D);
-#pragma unroll 4
-    for (int c = c0 + warp % WPR; c <= c1; c += WPR) {
-      const long long part = (long long)(2 * c + (c == c0 ? 1 : 0)) * R + r;
-      const float2 ml = parts_ml[part];
-      const float* src = p.ws + part * D + lane * C;
-      const float mn = fmaxf(top, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-      const float f0 = ex2(top - ref), f1 = ex2(ml.x - ref);
-      l = fmaf(l, f0, ml.y * f1);
+  if (c0 >= 0) {
+    const float2* parts_ml = reinterpret_cast<const float2*>(p.ws + attn_ml_at(p.grid, R, D));
+    // four parts at a time, their loads side by side whether or not there are four
+    for (int c = c0 + warp % WPR; c <= c1; c += 4 * WPR) {
+      float2 ml[4];
+      float x[4][C];
 #pragma unroll
-      for (int i = 0; i < C; ++i) acc[i] = fmaf(acc[i], f0, src[i] * f1);
+      for (int k = 0; k < 4; ++k) {
+        const int ck = c + k * WPR;
+        const bool there = ck <= c1;
+        const long long part = (long long)(2 * ck + (ck == c0 ? 1 : 0)) * R + r;
+        ml[k] = there ? parts_ml[part] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int i = 0; i < C; ++i) x[k][i] = there ? p.ws[part * D + lane * C + i] : 0.0f;
+      }
+      float mn = top;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mn = fmaxf(mn, ml[k].x);
+      const float ref = mn == -INFINITY ? 0.0f : mn, f0 = ex2(top - ref);
+      l *= f0;
+#pragma unroll
+      for (int i = 0; i < C; ++i) acc[i] *= f0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = ex2(ml[k].x - ref);
+        l = fmaf(ml[k].y, f, l);
+#pragma unroll
+        for (int i = 0; i < C; ++i) acc[i] = fmaf(x[k][i], f, acc[i]);
+      }
       top = mn;
     }
   }
@@ -826,7 +836,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int 
       for (int i = 0; i < C; ++i) acc[i] = fmaf(s_acc[warp + w][lane * C + i], f, acc[i]);
     }
   }
-  if (!cut) return;
+  if (c0 < 0) return;
+  const int token = u.first + (u.row0 + r) / p.group, h = u.head * p.group + (u.row0 + r) % p.group;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   T* dst = reinterpret_cast<T*>(p.out) + token * p.o_tok + h * p.o_head + lane * C;
   if constexpr (sizeof(T) == 2 && C >= 2) {
@@ -840,7 +851,70 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int 
 #pragma unroll
     for (int i = 0; i < C; ++i) dst[i] = Elem<T>::from_float(acc[i] * inv);
   }
-  if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+  if (p.lse && lane == 0) p.lse[(long long)token * p.Hq + h] = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+
+// Joins the parts of the units that attn_kernel cut, in the order of the CTAs.  WPR warps (1, 2, 4 or 8) of the CTA's 8
+// share an output row.  Which rows there are stands in what attn_kernel's CTAs left (AttnCut): every CTA here adds their
+// counts up and takes its place among the cut rows, however many sequences the call has and wherever their rows lie.
+// That is a load and a scan of the counts in front of the parts' loads (one sequence of 1000 tokens, 4 kv heads of 128:
+// 8.4 us).  Finding the same out from the lengths before the wait hides it (7.2 us), but only the wait promises that those
+// can be seen, and each row's warps then add up the work of all sequences (1024 sequences of up to 600 tokens, 8 kv
+// heads: 285 us instead of 245).
+template <typename T, int D, int WPR>
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParams p, int r_shift) {
+  constexpr int RPC = 8 / WPR;
+  const int R = 1 << r_shift;
+  __shared__ float s_acc[WPR > 1 ? 8 : 1][D];
+  __shared__ float2 s_ml[8];
+  __shared__ int s_rows[8];
+  __shared__ int3 s_at[RPC];                                          // what join_row takes
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  if (threadIdx.x < RPC) s_at[threadIdx.x].x = -1;
+  pdl_wait();
+  const int* const words = reinterpret_cast<const int*>(p.ws + attn_span_at(p.grid, R, D));
+  const int c_own = threadIdx.x * 4;
+  int span[4] = {0, 0, 0, 0};
+  if (c_own < p.grid) {                                               // padded to a multiple of four
+    const int4 v = *reinterpret_cast<const int4*>(words + c_own);
+    span[0] = v.x;
+    if (c_own + 1 < p.grid) span[1] = v.y;
+    if (c_own + 2 < p.grid) span[2] = v.z;
+    if (c_own + 3 < p.grid) span[3] = v.w;
+  }
+  const int mine = (span[0] & 255) + (span[1] & 255) + (span[2] & 255) + (span[3] & 255);
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) s_rows[warp] = incl;
+  __syncthreads();
+  int before = incl - mine, total = 0;                                // cut rows before this thread's, and all of them
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before += w < warp ? s_rows[w] : 0;
+    total += s_rows[w];
+  }
+  // One round, but where spans that do not fit make sequences share rows: then there can be more cut rows than rows.
+  for (int first = (int)blockIdx.x * RPC; first < total; first += (int)gridDim.x * RPC) {
+    int at = before - first;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = span[i] & 255;
+      for (int k = max(at, 0); k < min(at + n, RPC); ++k) s_at[k] = make_int3(c_own + i, k - at, span[i] >> 8);
+      at += n;
+    }
+    __syncthreads();
+    const int3 row = s_at[warp / WPR];
+    join_row<T, D, WPR>(p, R, row.x, row.y, row.z, s_acc, s_ml);
+    if (first + (int)gridDim.x * RPC >= total) break;
+    __syncthreads();
+    if (threadIdx.x < RPC) s_at[threadIdx.x].x = -1;
+    __syncthreads();
+  }
 }
 
 }  // namespace b200moe
