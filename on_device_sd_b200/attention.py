@@ -56,6 +56,9 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     its last row sees all context_lens[b] keys (the verify step).  max_query_len, the longest span, picks the row tile; any
     value gives right results.  scale defaults to D ** -0.5.
 
+    Scores, softmax and sums are fp32.  With 16-bit tensors each probability is rounded to their type before its product with
+    the value (half a step: 2^-8 of the weighted mean of |v| in bf16, 2^-11 in fp16), and the output once more.
+
     Returns out [T, heads, D] (with return_lse also the fp32 log-sum-exp [T, heads]).  A row that sees no key gives zeros
     and -inf; rows behind query_start[B] are not written (nor initialised unless `out` was given).  `out` may be `query`."""
     return load_step().paged_attention(query, k_cache, v_cache, block_tables, context_lens, query_start, max_query_len, scale, out, return_lse, status)
