@@ -26,7 +26,8 @@ def rotary_table(head_dim: int, max_position: int, base: float = 1e6, device: Op
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, *,
                   status: Optional[torch.Tensor] = None) -> None:
     """key, value [T, kv_heads, D] -> rows slot_mapping[t] of the caches; slot -1 stores nothing (the reference's function of
-    this name, demo/src/layers/attention.py:56-79).  The slots of one call are distinct."""
+    this name, demo/src/layers/attention.py:56-79).  The slots of one call are distinct, k_cache and v_cache share no memory,
+    and key and value are not rows that the call writes."""
     load_step().store_kv(None, key, value, None, None, k_cache, v_cache, slot_mapping, None, None, 0.0, None, status)
 
 
@@ -39,7 +40,7 @@ def rope_store_kvcache(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
 
     query [T, heads, D], key and value [T, kv_heads, D] may be views of one projection row; positions and slot_mapping are
     int64 or int32 [T]; cos_sin is rotary_table's.  Returns the rotated queries [T, heads, D] (`out` when given, which may
-    be `query` itself).  fp32 inside, each output rounded once."""
+    be `query` itself and otherwise shares no memory with the other tensors).  fp32 inside, each output rounded once."""
     if query is None or cos_sin is None or positions is None:
         raise ValueError("rope_store_kvcache needs query, positions and cos_sin (store_kvcache stores keys and values alone)")
     return load_step().store_kv(query, key, value, positions, cos_sin, k_cache, v_cache, slot_mapping, q_norm_weight, k_norm_weight, eps, out, status)
@@ -60,5 +61,6 @@ def paged_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     the value (half a step: 2^-8 of the weighted mean of |v| in bf16, 2^-11 in fp16), and the output once more.
 
     Returns out [T, heads, D] (with return_lse also the fp32 log-sum-exp [T, heads]).  A row that sees no key gives zeros
-    and -inf; rows behind query_start[B] are not written (nor initialised unless `out` was given).  `out` may be `query`."""
+    and -inf; rows behind query_start[B] are not written (nor initialised unless `out` was given).  `out` may be
+    `query` itself; otherwise it shares no memory with it or the caches."""
     return load_step().paged_attention(query, k_cache, v_cache, block_tables, context_lens, query_start, max_query_len, scale, out, return_lse, status)

@@ -57,7 +57,7 @@ def nvcc_path() -> str:
 
 def _build_step(force: bool, verbose: bool) -> None:
     src = CSRC / "bindings.cpp"
-    deps = (src, PKG.parent / "include" / "b200moe.h", Path(__file__))
+    deps = (src, CSRC / "overlap.h", PKG.parent / "include" / "b200moe.h", Path(__file__))
     if not force and STEP.exists() and all(p.stat().st_mtime <= STEP.stat().st_mtime for p in deps):
         return
     import sysconfig

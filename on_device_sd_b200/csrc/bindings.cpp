@@ -16,6 +16,7 @@
 #include <string>
 
 #include "../../include/b200moe.h"
+#include "overlap.h"
 
 namespace {
 
@@ -75,6 +76,24 @@ int64_t step(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stri
 void own_places(const at::Tensor& t, const char* name) {
   for (int64_t d = 0; d < t.dim(); ++d)
     if (t.size(d) > 1 && t.stride(d) == 0) refuse(PyExc_ValueError, std::string(name) + " is written and must not be an expanded tensor, got strides " + shape_text(t.strides()));
+}
+
+// --- shared memory ----------------------------------------------------------------------------
+// The rows (last dimension) of a tensor of 3 or 4 dimensions.
+b200moe::StridedRows rows_of(const at::Tensor& t) {
+  b200moe::StridedRows r;
+  const int64_t e = (int64_t)t.element_size(), last = t.dim() - 1;
+  r.base = (uintptr_t)t.data_ptr();
+  r.width = t.size(last) * e;
+  for (int64_t d = 0; d < last; ++d) r.axis(t.size(d), t.stride(d) * e);
+  return r;
+}
+// A kernel reads some rows after it has written others: what is written may not partly cover what is read.
+void apart(const b200moe::StridedRows& out, const char* out_name, const at::Tensor& t, const char* name, bool may_be_same) {
+  const b200moe::StridedRows r = rows_of(t);
+  if (may_be_same && out.same(r)) return;
+  if (b200moe::rows_meet(out, r))
+    refuse(PyExc_ValueError, std::string(out_name) + " shares memory with " + name + (may_be_same ? "; it may be the same tensor or a separate one, nothing between" : ""));
 }
 
 // --- checks -----------------------------------------------------------------------------------
@@ -193,6 +212,7 @@ PyObject* store_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (kc.size(2) != hk) refuse(PyExc_ValueError, "the caches hold " + std::to_string(kc.size(2)) + " key-value heads, key and value " + std::to_string(hk));
     own_places(kc, "k_cache");
     own_places(vc, "v_cache");
+    apart(rows_of(kc), "k_cache", vc, "v_cache", false);
     heads_contiguous(key, "key");
     heads_contiguous(value, "value");
     s.slots = index(tensor(a[7], "slot_mapping"), "slot_mapping", dev, T, &s.slots_are_int64);
@@ -208,6 +228,14 @@ PyObject* store_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
         refuse(PyExc_ValueError, "query must be [" + std::to_string(T) + ", heads, " + std::to_string(D) + "], got " + shape_text(query->sizes()));
       heads_contiguous(*query, "query");
       out = output(a[11], dev, dt, query->sizes());
+      if (a[11] != Py_None) {
+        const b200moe::StridedRows o = rows_of(out);
+        apart(o, "out", *query, "query", true);
+        apart(o, "out", key, "key", false);
+        apart(o, "out", value, "value", false);
+        apart(o, "out", kc, "k_cache", false);
+        apart(o, "out", vc, "v_cache", false);
+      }
       s.query = query->data_ptr(); s.query_out = out.data_ptr(); s.num_heads = int32(query->size(1), "heads");
       s.q_token_stride = step(*query, 0); s.q_head_stride = step(*query, 1); s.o_token_stride = step(out, 0); s.o_head_stride = step(out, 1);
     }
@@ -271,6 +299,12 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.scale = (float)scale;
     const c10::cuda::CUDAGuard guard(dev);
     at::Tensor out = output(a[8], dev, dt, query.sizes()), lse, ws;
+    if (a[8] != Py_None) {
+      const b200moe::StridedRows o = rows_of(out);
+      apart(o, "out", query, "query", true);
+      apart(o, "out", kc, "k_cache", false);
+      apart(o, "out", vc, "v_cache", false);
+    }
     s.out = out.data_ptr(); s.o_token_stride = step(out, 0); s.o_head_stride = step(out, 1);
     if (with_lse) {
       lse = empty(dev, at::kFloat, {T, hq});
