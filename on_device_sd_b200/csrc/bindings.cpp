@@ -347,6 +347,8 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t drafts = tokens.size(0), B = sample.size(0), vocab = target.size(1), longest = integer(a[6], "max_draft_len");
     if (longest < 0) refuse(PyExc_ValueError, "max_draft_len must not be negative");
     if (vocab == 0) refuse(PyExc_ValueError, "the vocabulary is empty");
+    if (target.size(0) < B)   // the drafts' own rows depend on draft_start, which the kernel reads: drafts behind its end need none
+      refuse(PyExc_ValueError, "target_probs must have a row for every draft and one more per sequence, got " + std::to_string(target.size(0)) + " rows for " + std::to_string(B) + " sequences");
     s.draft_tokens = (const int64_t*)vec(tokens, "draft_tokens", dev, at::kLong, drafts);
     s.sample_uniform = (const float*)vec(sample, "sample_uniform", dev, at::kFloat, B);
     s.accept_uniform = (const float*)vec(accept, "accept_uniform", dev, at::kFloat, drafts);

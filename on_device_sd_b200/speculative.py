@@ -23,5 +23,7 @@ def verify_draft(draft_tokens: torch.Tensor, target_probs: torch.Tensor, draft_p
     drawn from max(p_j - q_j, 0), after a fully accepted span from the last row, both by inverse cumulative sum at
     sample_uniform[b].  draft_probs None means greedy drafts: q is 1 on the drafted token.  Rows of `tokens` hold the accepted
     tokens, the drawn one, then -1.  Both uniforms are float32; probabilities float32, float16 or bfloat16 (one type for
-    both), after the caller's temperature and top-k / top-p.  Errors and `status` as in attention.py."""
+    both), after the caller's temperature and top-k / top-p.  Errors and `status` as in attention.py; a sequence whose rows
+    do not fit the tensors (fewer target rows than draft_start[b+1] + b + 1 among them, a span longer than max_draft_len)
+    gets a row of -1 and 0 accepted, and shows only there and in `status`."""
     return load_step().verify_draft(draft_tokens, target_probs, draft_probs, accept_uniform, sample_uniform, draft_start, max_draft_len, status)
