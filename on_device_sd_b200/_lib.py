@@ -148,8 +148,11 @@ def load_step():
         if not STEP_PATH.exists():
             raise ImportError(f"{STEP_PATH} is missing: build it with `python -m on_device_sd_b200.build`. There is no fallback path.")
         load()
-        import torch  # noqa: F401  (the libraries that _step.so is linked to)
         from importlib import import_module
+
+        from .build import built_for, step_tag   # imports torch: the libraries that _step.so is linked to
+        if built_for(STEP_PATH) != step_tag():
+            raise ImportError(f"{STEP_PATH} was built for {built_for(STEP_PATH)}, this is {step_tag()}: rebuild it with `python -m on_device_sd_b200.build`")
         _step = import_module("on_device_sd_b200._step")
     return _step
 

@@ -18,6 +18,12 @@
 #include "../../include/b200moe.h"
 #include "overlap.h"
 
+// What this file was compiled against; build.py and _lib.py read it from the file before they load it.
+#ifndef B200MOE_STEP_TAG
+#error "compile with build.py, which names the torch and the Python that this is built against"
+#endif
+extern "C" __attribute__((used, visibility("default"))) const char b200moe_step_tag[] = "b200moe_step built for <" B200MOE_STEP_TAG ">";
+
 namespace {
 
 struct Refusal {                     // becomes a Python exception
