@@ -286,6 +286,10 @@ extern "C" int b200moe_paged_attention(const b200moe_paged_attention_args* a, vo
   if (max_context > (1ll << 30)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: block tables span more than 2^30 slots", who);
   // the join's grid and the row numbers are 32-bit
   if ((int64_t)a->num_tokens * a->num_heads > (1ll << 30)) return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: more than 2^30 tokens x heads", who);
+  // work items are tiles of at least 32 keys x 16 rows, numbered in 64 bits and multiplied by the grid (at most 2^10)
+  const double rows16 = (double)a->num_tokens * (a->num_heads / a->num_kv_heads) / 16 + std::min(a->num_tokens, a->num_seqs);
+  if (rows16 * a->num_kv_heads * ((double)max_context / 32 + 1 + kUnitCost) > 4503599627370496.0)
+    return b200moe_fail_global(B200MOE_E_UNSUPPORTED, "%s: more than 2^52 tiles of work", who);
   int dev;
   if (int rc = current_device(who, &dev)) return rc;
   AttnParams p = {};
