@@ -131,14 +131,16 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
     while ((1ll << sh) < p->block_size) ++sh;
     p->page_shift = 31 + sh;
     p->page_mul = (unsigned)((1ull << (31 + sh)) / (unsigned)p->block_size + 1);
+    const long long rows = (long long)p->T * p->Hq;
+    p->cuts = p->split && rows > 8 * 148;
     e = p->block_size % 16 == 0 ? start<true>(*p, grid, dev, s) : start<false>(*p, grid, dev, s);
     if (e != cudaSuccess || !p->split) return e;
-    const long long rows = std::min((long long)p->T * p->Hq, (long long)(full - 1) * S::R);   // no more are cut: one unit a CTA
     // Few rows are cut into many parts each: up to eight warps per row, in up to two CTAs of eight on every SM.
-    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, kJoinThreads, 0, s, *p, S::R_SHIFT);
-    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), kJoinThreads, 0, s, *p, S::R_SHIFT);
-    if (rows <= 8 * 148) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), kJoinThreads, 0, s, *p, S::R_SHIFT);
-    return launch(attn_join_kernel<T, D, 1>, (unsigned)((rows + 7) / 8), kJoinThreads, 0, s, *p, S::R_SHIFT);
+    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R_SHIFT);
+    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), 256, 0, s, *p, S::R_SHIFT);
+    if (!p->cuts) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), 256, 0, s, *p, S::R_SHIFT);
+    // no more rows are cut than there are, or than the CTAs can begin units of
+    return launch(attn_join_cuts_kernel<T, D>, (unsigned)((std::min(rows, (long long)(full - 1) * S::R) + 7) / 8), kJoinThreads, 0, s, *p, S::R_SHIFT);
   }
 };
 

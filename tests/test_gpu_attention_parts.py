@@ -54,7 +54,8 @@ def test_rows_between_the_sequences_of_a_cut_call(dtype):
     assert (out[c.starts[-1]:] == 5.0).all()
 
 
-@pytest.mark.parametrize("batch, span, context, heads", [(128, 8, 700, (32, 4, 64)), (1000, 1, 300, (8, 8, 64)), (300, 1, 1500, (4, 1, 32)), (2, 1, 60000, (32, 8, 64))])
+@pytest.mark.parametrize("batch, span, context, heads", [(128, 8, 700, (32, 4, 64)), (1000, 1, 300, (8, 8, 64)), (300, 1, 1500, (4, 1, 32)), (2, 1, 60000, (32, 8, 64)),
+                                                         (40, 1, 3000, (4, 1, 64)), (33, 4, 900, (4, 2, 32)), (100, 1, 2000, (8, 1, 256))])
 def test_cut_batches_of_all_sizes(batch, span, context, heads):
     """From far more units than CTAs to far fewer; the same call gives the same bits."""
     hq, hk, d = heads
