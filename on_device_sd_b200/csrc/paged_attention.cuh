@@ -69,9 +69,14 @@ struct AttnSeq {
   int first, n, ctx;               // first query row, new tokens, keys
   int row_tiles, tiles;
 };
-template <bool FRESH = false>                      // FRESH: not from L1
+template <bool AGAIN = false>                      // AGAIN: loaded here and now, whatever has been loaded before
 __device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b, int r_shift) {   // a row tile holds 1 << r_shift rows
-  auto get = [](const int* at) { return FRESH ? __ldcv(at) : *at; };
+  auto get = [](const int* at) {
+    if constexpr (!AGAIN) return *at;
+    int v;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
+    return v;
+  };
   AttnSeq s;
   s.first = b; s.n = 1;
   s.ctx = get(p.context + b);
