@@ -29,6 +29,15 @@ int current_device(const char* who, int* dev) {
   return B200MOE_OK;
 }
 
+int sm_count(int dev, cudaError_t* err) {
+  static std::atomic<int> known[kMaxDevices];      // two threads that ask at once store the same number
+  int n = known[dev].load(std::memory_order_acquire);
+  if (n) return n;
+  *err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (*err == cudaSuccess) known[dev].store(n, std::memory_order_release);
+  return n;
+}
+
 // Every kernel here waits for its predecessor itself (pdl_wait), so it may be launched while that one drains.
 template <typename... Params, typename... Args>
 cudaError_t launch(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
@@ -48,21 +57,24 @@ cudaError_t launch(void (*kernel)(Params...), unsigned grid, unsigned threads, s
 // ---------------------------------------------------------------------------------------------
 // b200moe_store_kv
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D> cudaError_t launch_store(const StoreKvParams& p, cudaStream_t s) {
+template <typename T, int D> cudaError_t launch_store(const StoreKvParams& p, int dev, cudaStream_t s) {
   constexpr int L = D / 16;
   const int heads = p.Hq + 2 * p.Hkv;
-  // One head per lane group until that fills the GPU about twice (148 SMs x 2048 threads), four from there on.
-  const bool wide = (long long)p.T * heads * L >= 2ll * 148 * 2048;
+  cudaError_t e = cudaSuccess;
+  const int sms = sm_count(dev, &e);
+  if (e != cudaSuccess) return e;
+  // One head per lane group until that fills the GPU about twice (SMs x 2048 threads), four from there on.
+  const bool wide = (long long)p.T * heads * L >= 2ll * sms * 2048;
   const long long groups = (long long)p.T * (wide ? (heads + 3) / 4 : heads);
   const unsigned grid = (unsigned)((groups * L + kStoreThreads - 1) / kStoreThreads);
   return wide ? launch(store_kv_kernel<T, D, 4>, grid, kStoreThreads, 0, s, p) : launch(store_kv_kernel<T, D, 1>, grid, kStoreThreads, 0, s, p);
 }
-template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, cudaStream_t s) {
+template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, int dev, cudaStream_t s) {
   switch (D) {
-    case 32: return launch_store<T, 32>(p, s);
-    case 64: return launch_store<T, 64>(p, s);
-    case 128: return launch_store<T, 128>(p, s);
-    default: return launch_store<T, 256>(p, s);
+    case 32: return launch_store<T, 32>(p, dev, s);
+    case 64: return launch_store<T, 64>(p, dev, s);
+    case 128: return launch_store<T, 128>(p, dev, s);
+    default: return launch_store<T, 256>(p, dev, s);
   }
 }
 
@@ -85,15 +97,6 @@ struct AttnPlan {
   int64_t ws_bytes = 0;            // 0: units are not cut
 };
 
-int sm_count(int dev, cudaError_t* err) {
-  static std::atomic<int> known[kMaxDevices];      // two threads that ask at once store the same number
-  int n = known[dev].load(std::memory_order_acquire);
-  if (n) return n;
-  *err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  if (*err == cudaSuccess) known[dev].store(n, std::memory_order_release);
-  return n;
-}
-
 // MINB CTAs fit an SM: they are what the grid holds, so that all parts of a call run at once.
 template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int REGB = MINB> struct AttnVariant {
   using S = AttnShape<T, D, MT, RG, KG, STAGES>;
@@ -111,7 +114,7 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
   }
   static cudaError_t run(AttnParams* p, int dev, AttnPlan* plan, cudaStream_t s, bool plan_only) {
     cudaError_t e = cudaSuccess;
-    const int full = MINB * sm_count(dev, &e);
+    const int sms = sm_count(dev, &e), full = MINB * sms;
     if (e != cudaSuccess) return e;
     // as far as comparisons need them
     const long long row_tiles = std::min(((long long)p->span * p->group + S::R - 1) / S::R, 1ll << 20);
@@ -132,12 +135,12 @@ template <typename T, int D, int MT, int RG, int KG, int STAGES, int MINB, int R
     p->page_shift = 31 + sh;
     p->page_mul = (unsigned)((1ull << (31 + sh)) / (unsigned)p->block_size + 1);
     const long long rows = (long long)p->T * p->Hq;
-    p->cuts = p->split && rows > 8 * 148;
+    p->cuts = p->split && rows > 8 * sms;
     e = p->block_size % 16 == 0 ? start<true>(*p, grid, dev, s) : start<false>(*p, grid, dev, s);
     if (e != cudaSuccess || !p->split) return e;
     // Few rows are cut into many parts each: up to eight warps per row, in up to two CTAs of eight on every SM.
-    if (rows <= 2 * 148) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R_SHIFT);
-    if (rows <= 4 * 148) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), 256, 0, s, *p, S::R_SHIFT);
+    if (rows <= 2 * sms) return launch(attn_join_kernel<T, D, 8>, (unsigned)rows, 256, 0, s, *p, S::R_SHIFT);
+    if (rows <= 4 * sms) return launch(attn_join_kernel<T, D, 4>, (unsigned)((rows + 1) / 2), 256, 0, s, *p, S::R_SHIFT);
     if (!p->cuts) return launch(attn_join_kernel<T, D, 2>, (unsigned)((rows + 3) / 4), 256, 0, s, *p, S::R_SHIFT);
     // no more rows are cut than there are, or than the CTAs can begin units of
     return launch(attn_join_cuts_kernel<T, D>, (unsigned)((std::min(rows, (long long)(full - 1) * S::R) + 7) / 8), kJoinThreads, 0, s, *p, S::R_SHIFT);
@@ -235,9 +238,9 @@ extern "C" int b200moe_store_kv(const b200moe_store_kv_args* a, void* stream) {
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   switch (dt) {
-    case B200MOE_F32: e = dispatch_store<float>(p, a->head_dim, s); break;
-    case B200MOE_F16: e = dispatch_store<__half>(p, a->head_dim, s); break;
-    default: e = dispatch_store<__nv_bfloat16>(p, a->head_dim, s); break;
+    case B200MOE_F32: e = dispatch_store<float>(p, a->head_dim, dev, s); break;
+    case B200MOE_F16: e = dispatch_store<__half>(p, a->head_dim, dev, s); break;
+    default: e = dispatch_store<__nv_bfloat16>(p, a->head_dim, dev, s); break;
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
