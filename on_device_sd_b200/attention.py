@@ -3,9 +3,10 @@ embedding in the same launch) and the attention of new tokens, single ones (draf
 
 The cache tensors are the reference's, [num_blocks, block_size, kv_heads, head_dim] (demo/src/memory/paged_kv_cache.py:228),
 and stay the caller's.  All calls run on the current stream of their tensors' device, never synchronise and can be
-captured into CUDA graphs.  `status`, where given, is an int32 tensor of one element on the same device that the kernels
-OR DEV_* bits into (include/b200moe.h); the caller zeroes and reads it.  Arguments are checked in csrc/bindings.cpp:
-ValueError / TypeError for tensors that do not fit together, B200MoEError for what the library refuses."""
+captured into CUDA graphs; there are no gradients.  `status`, where given, is an int32 tensor of one element on the
+same device that the kernels OR DEV_* bits into (include/b200moe.h); the caller zeroes and reads it.  Arguments are
+checked in csrc/bindings.cpp: ValueError / TypeError for tensors that do not fit together, B200MoEError for what the
+library refuses."""
 from __future__ import annotations
 
 from typing import Optional, Tuple, Union

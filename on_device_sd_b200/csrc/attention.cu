@@ -83,11 +83,15 @@ template <typename T> cudaError_t dispatch_store(const StoreKvParams& p, int D, 
 // ---------------------------------------------------------------------------------------------
 // Whether a call's units are cut along the cache over the whole grid, from what the host knows: B sequences of at most
 // max_blocks * block_size slots.  Uncut, a unit belongs to one CTA, which takes about 0.9 us for a tile when it has the
-// time to itself; cut, a second kernel joins the parts.  16-bit types, heads of 128, 4 kv heads, us uncut / cut: one
-// sequence of 33 slots 5.5 / 6.1, of 120 6.4 / 6.8, of 250 8.0 / 6.7 (tables are as wide as the pages, lengths lie
-// anywhere below: on average 4 tiles break even); 16 sequences of 250 8.2 / 9.0.  Units that just fill the GPU once gain
-// longer: 64 sequences of 500 13.3 / 16.4; of 1000, cut, 29.1; with 8 kv heads, more units than fit at once, 29.9 / 29.7 at
-// 500.  fp32: one sequence of 60 slots 5.9 / 6.6; past a tile its products alone take longer than the join.
+// time to itself (fp32 3.2); cut, a second kernel joins the parts, and the division costs every unit kUnitCost.  us uncut /
+// cut, all lengths equal, 4 kv heads of 128 with 8 queries each:
+//   16-bit, one token a sequence   1 x 33 slots 5.4 / 6.5, 120 6.3 / 6.6, 250 7.9 / 6.6;  16 x 250 8.2 / 9.0, 500 11.3 / 10.0
+//   16-bit, spans of 5             1 x 120 8.9 / 9.0, 250 10.9 / 9.2, 500 15.0 / 9.8;     16 x 250 11.6 / 14.6, 500 15.7 / 17.2
+//   units that just fill the GPU   64 x 250 9.8 / 13.8, 500 13.4 / 17.9, 1000 26.9 / 30.2
+//   fp32                           1 x 60 8.1 / 9.5, 120 11.4 / 9.3;  16 x 120 11.5 / 14.3, 500 30.8 / 23.2;  64 x 500 62 / 65
+// One sequence breaks even at 2 or 3 tiles, several at 6 to 20, but lengths lie anywhere below the table's width, and of ragged
+// ones the longest sets the uncut time: 4 tiles, 8 where the units just fill the GPU, are between the two.  So short spans
+// of one sequence pay up to 2 us (250 slots), and equal lengths past 8 tiles, or in fp32 past one, up to 3 or 4.
 constexpr int kUncutTiles = 4, kUncutTilesFull = 8, kUncutTilesF32 = 1;
 // What beginning a unit costs a CTA, in tiles of 64 keys, for the equal division of the work.  (32 spans over 100..2500
 // tokens: 55 us at 0, 48 at 1, 44 at 2, 43 at 3; equal lengths do not care.)

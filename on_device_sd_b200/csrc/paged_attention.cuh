@@ -17,22 +17,24 @@
 // they fill with cp.async: no barrier of the CTA in the loop (with two row groups, one of 64 threads per stage).  When a
 // unit ends, the loads of the next begin before the groups' results meet in the free slots of their rings.
 // 16-bit types multiply on mma.sync m16n8k16: rows (padded to 16) x keys, accumulators and the softmax in registers.
-// With 16 rows the tensor pipe is 19 % busy when HBM is saturated, with 32 rows 33 %; the hand-over through tensor memory
+// With 16 rows the tensor pipe is 19 % busy when HBM is saturated, with 32 rows 36 %; the hand-over through tensor memory
 // that tcgen05 needs between the two products would lengthen the path of the few rows that decoding has.  Past 32 rows
-// per kv head it would pay (the cache is then read once per 32 rows, from L2 at best): not built.
-// fp32 multiplies on the CUDA cores.
+// per kv head it would pay (the cache is then read once per 32 rows, from L2 at best): not built.  A prompt of 2048 tokens, 32
+// query heads on 4, takes 478 us, 72 TFLOP/s, a twentieth of what the tensor cores give matrix products.
+// fp32 multiplies on the CUDA cores (16 sequences of 300..6000 tokens 95 us, 2.6 times the bytes' time).
 //
 // Roundings: scores, softmax, sums and accumulators are fp32; p is rounded to the cache's type for the second product
 // (the operand type of the tensor cores; the sum l uses the same unrounded p), outputs are rounded once.  That costs at
 // most half a step of the type, 2^-8 (bf16) or 2^-11 of sum_j p_j |v_j| / l, besides the output's own; fp32 rounds no p.
 //
-// Measured on B200, device time back to back, heads of 128: 32 sequences of 21000 tokens, 8 kv heads of 4 queries 405 us
-// (6.8 TB/s, the copy rate), with spans of 8 tokens 430 us; one sequence of 131071, 4 kv heads 50.8 us (5.3 TB/s); 16 of
-// 300..6000 25.4 us (4.7 TB/s); 64 spans of 1..5 tokens, 8 queries a kv head, over 800..16384 tokens 228 us.  What is
+// Measured on B200, device time back to back, heads of 128: 32 sequences of 21000 tokens, 8 kv heads of 4 queries 414 us
+// (6.7 TB/s, the copy rate), with spans of 8 tokens 420; one sequence of 131071, 4 kv heads 48.6 us (5.5 TB/s); 16 of
+// 300..6000 25.5 us (4.7 TB/s); 64 spans of 1..5 tokens, 8 queries a kv head, over 800..16384 tokens 233 us.  What is
 // left there is fixed cost: about 5 us from the launch to the first products (lengths, page table and cache are three
-// dependent loads), about 3 us for the join.  A stage of 16 keys is some 1600 cycles of dependent instructions for its
-// warp whatever is in flight, which eight warps an SM hide for 16 rows and just about for 32.  Slower were: bulk copies of a
-// row per lane (by 10 to 30 %), rows padded in shared memory instead of permuted (3 to 9 %), a deeper ring (nothing).
+// dependent loads), 1.5 to 5 us for the join.  A stage of 16 keys is some 1600 cycles of dependent instructions for its
+// warp whatever is in flight, which eight warps an SM hide for 16 rows and just about for 32, where heads of 128 also
+// spill 48 bytes a thread (92 with pages that are no multiple of 16 slots).  Slower were: bulk copies of a row per lane (by
+// 10 to 30 %), rows padded in shared memory instead of permuted (3 to 9 %), a deeper ring (nothing).
 #pragma once
 #include <type_traits>
 
