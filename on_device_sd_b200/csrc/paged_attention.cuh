@@ -869,10 +869,27 @@ template <typename T, int D> __device__ __forceinline__ void join_store(const At
   if (p.lse && lane == 0) p.lse[(long long)j.token * p.Hq + j.h] = s.l == 0.0f ? -INFINITY : (s.top + log2f(s.l)) * 0.6931471805599453f;
 }
 
+// 64 bits that lengths which differ share by an accident of 2^-64.
+__device__ __forceinline__ unsigned long long join_digest(unsigned long long d, const AttnSeq& s) {
+  d = d * 0x9e3779b97f4a7c15ull + ((unsigned long long)(unsigned)s.ctx << 32 | (unsigned)s.first);
+  return d * 0xd1b54a32d192ed03ull + (unsigned)s.n;
+}
+__device__ __forceinline__ unsigned long long join_lengths(const AttnParams& p, int r_shift) {
+  unsigned long long d = 0;
+#pragma unroll 4
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + (int)(threadIdx.x & 31);
+    AttnSeq sq = {};
+    if (b < p.B) sq = attn_seq<true>(p, b, r_shift);
+    d = join_digest(d, sq);
+  }
+  return d;
+}
+
 // What became of an output row, from the lengths; by a whole warp.  Starts need not be in order (spans that fit nothing stand
 // between): the row belongs to the first sequence that holds it.
-// *seen: this lane's part of the lengths, for up to 32 sequences.
-__device__ __forceinline__ void join_find(const AttnParams& p, int r_shift, JoinRow* j, int3* seen) {
+// *seen: a digest of this lane's part of the lengths (join_lengths).
+__device__ __forceinline__ void join_find(const AttnParams& p, int r_shift, JoinRow* j, unsigned long long* seen) {
   const int lane = threadIdx.x & 31;
   long long all = 0, before = 0;   // of this lane's sequences: work, and work in front of the row's sequence
   int first = 0, n = 0, tiles = 0, row_tiles = 0, weight = 0;
@@ -885,7 +902,7 @@ __device__ __forceinline__ void join_find(const AttnParams& p, int r_shift, Join
       sq = attn_seq<true>(p, b, r_shift);
       w = attn_work(p, sq);
     }
-    *seen = make_int3(sq.first, sq.n, sq.ctx);
+    *seen = join_digest(*seen, sq);
     all += w;
     if (have) continue;
     const unsigned hit = __ballot_sync(0xffffffffu, j->token >= sq.first && j->token - sq.first < sq.n);
@@ -927,19 +944,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int 
   pdl_trigger();
   const unsigned row = blockIdx.x * RPC + warp / WPR;                 // (token, head), below 2^31
   JoinRow j = {0, -1, 0, (int)(row / (unsigned)p.Hq), (int)(row % (unsigned)p.Hq)};
-  int3 seen = make_int3(0, 0, 0);
+  unsigned long long seen = 0;
   if (j.token < p.T) join_find(p, r_shift, &j, &seen);
   pdl_wait();
   JoinParts<C> q;
   q.template load<D, WPR>(p, j, R, j.c0 + warp % WPR);
   if (j.token < p.T) {
-    bool changed = p.B > 32;
-    if (!changed) {
-      AttnSeq sq = {};
-      if (lane < p.B) sq = attn_seq<true>(p, lane, r_shift);
-      changed = __any_sync(0xffffffffu, sq.first != seen.x || sq.n != seen.y || sq.ctx != seen.z);
-    }
-    if (changed) {
+    if (__any_sync(0xffffffffu, join_lengths(p, r_shift) != seen)) {
       const JoinRow guess = j;
       join_find(p, r_shift, &j, &seen);
       if (j.c0 != guess.c0 || j.c1 != guess.c1 || j.r != guess.r) q.template load<D, WPR>(p, j, R, j.c0 + warp % WPR);
